@@ -300,6 +300,68 @@ int odbox_decode_nms_mixed(const float *anchors /*[N,4] or NULL*/, const void *r
                            int32_t *out_labels /*[B,max_ret]*/, int32_t *out_keep_anchor /*[B,max_ret]*/,
                            int32_t *out_count /*[B]*/, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- rows of class logits (no counterpart in the reference beyond the softmax of metric.py:19-20) ---- */
+
+/* logits: [rows, C] of `dtype` (ODBOX_DTYPE_*), the classes of a row side by side, rows row_stride ELEMENTS apart (>= C, or 0
+ * for one row read again and again); aligned to their element only.  Every result is computed in fp32 from the widened values.
+ * A logit of -inf is a class without probability.  A row whose logits are ALL -inf is empty: log-probabilities -inf, entropy 0,
+ * losses and gradients 0.  A row that holds a NaN or +inf gives NaN. */
+#define ODBOX_MAX_LOGITS 16777216   /* C: a class id is 24 bits of the selection key */
+#define ODBOX_MAX_TOP    128        /* top alternatives of a row, classes of a teacher's list */
+
+/* With z = logits / temperature: out_logprobs[row] = log softmax(z)[labels[row]] (0 for a label outside [0, C): a padded row),
+ * out_entropy[row] = -sum p log p in nats, and the top_k classes of largest logit, ordered by (logit descending, class ascending;
+ * NaN above everything), with their log-probabilities.  labels, out_logprobs, out_entropy may be NULL; the top outputs
+ * are [rows, top_k].  out_stats [rows, 4] (16-byte aligned, or NULL) is what the backward call needs.
+ * workspace: odbox_label_logprobs_workspace(rows, C, top_k) bytes (may be 0: then NULL will do), 16-byte aligned. */
+size_t odbox_label_logprobs_workspace(size_t rows, int C, int top_k);
+int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size_t row_stride,
+                         const int32_t *labels /*[rows] or NULL*/, int top_k, float temperature,
+                         float *out_logprobs /*[rows] or NULL*/, float *out_entropy /*[rows] or NULL*/,
+                         float *out_top_logprobs /*[rows,top_k]*/, int32_t *out_top_labels /*[rows,top_k]*/,
+                         float *out_stats /*[rows,4] or NULL*/, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Its gradient, grad [rows, C] of the logits' dtype, contiguous, rounded once:
+ *   d logits_i = (1/T) [ sum_j g_j [i = id_j] - p_i (sum_j g_j + gH (log p_i + H)) ]
+ * over the label's upstream value and those of the top alternatives (at their fixed classes); each upstream may be NULL.
+ * logits, labels, temperature and stats are the forward call's. */
+int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, int C, size_t row_stride,
+                                  const int32_t *labels /*[rows] or NULL*/, int top_k,
+                                  const int32_t *top_labels /*[rows,top_k] or NULL*/, float temperature,
+                                  const float *stats /*[rows,4]*/, const float *upstream_logprobs /*[rows] or NULL*/,
+                                  const float *upstream_entropy /*[rows] or NULL*/,
+                                  const float *upstream_top /*[rows,top_k] or NULL*/, void *grad, void *stream);
+
+/* Distillation from the K classes a teacher ranks best.  teacher_labels [rows, K] are their ids (an id outside [0, C) is an
+ * unused place; an id listed twice counts twice), teacher_logprobs [rows, K] their log-probabilities at the SAME temperature
+ * (what odbox_label_logprobs writes).  With q the teacher's and p = softmax(logits / T) the student's probabilities
+ *   loss[row] = w T^2 [ sum_k q_k (log q_k - log p[id_k]) + rest ]
+ * ODBOX_REST_RENORMALISE: q is renormalised over the list (any common shift of the teacher's values cancels), rest = 0.
+ * ODBOX_REST_BUCKET: q = exp(teacher_logprobs) and all classes off the list form one more class:
+ *   rest = q0 (log q0 - log p0), q0 = max(0, 1 - sum q), p0 = the student's mass off the list; left out where the student has none.
+ * row_weights w [rows] or NULL (all 1); a row of weight 0 is ignored: its logits are not read, its loss and gradient are 0.
+ * out_rows [rows] or NULL: the row losses.  out_loss [1] or NULL: scale * their sum, summed in a fixed order (not both NULL).
+ * grad [rows, C] or NULL: the gradient of scale * the sum, of the logits' dtype, contiguous.
+ * out_stats [rows, 4] (16-byte aligned, or NULL) is what the backward call needs.
+ * workspace: odbox_distill_loss_workspace(rows, C, K) bytes, 16-byte aligned. */
+#define ODBOX_REST_RENORMALISE 0
+#define ODBOX_REST_BUCKET      1
+size_t odbox_distill_loss_workspace(size_t rows, int C, int K);
+int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t row_stride,
+                       const float *teacher_logprobs /*[rows,K]*/, const int32_t *teacher_labels /*[rows,K]*/, int K,
+                       float temperature, int rest, const float *row_weights /*[rows] or NULL*/, float scale,
+                       float *out_rows /*[rows] or NULL*/, float *out_loss /*[1] or NULL*/,
+                       float *out_stats /*[rows,4] or NULL*/, void *grad /*[rows,C] or NULL*/,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* The gradient alone, from the forward call's statistics: scale * upstream * d loss[row] / d logits, upstream one device scalar
+ * (upstream_rows = 0) or one value a row (upstream_rows != 0). */
+int odbox_distill_loss_backward(const void *logits, int dtype, size_t rows, int C, size_t row_stride,
+                                const float *teacher_logprobs /*[rows,K]*/, const int32_t *teacher_labels /*[rows,K]*/, int K,
+                                float temperature, int rest, const float *row_weights /*[rows] or NULL*/, float scale,
+                                const float *stats /*[rows,4]*/, const float *upstream /*[1] or [rows]*/, int upstream_rows,
+                                void *grad /*[rows,C]*/, void *stream);
+
 /* ---- evaluation side: the step after the all-gather of detections ---- */
 
 /* evaluate.py:14-28 _COCO_result / :31-55 _COCO_gt_annot: xyxy -> (x, y, w, h) with fp32 w = x1-x0,

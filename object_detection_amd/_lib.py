@@ -47,6 +47,12 @@ SIGNATURES = {
     'odbox_set_nms_tier': (_i, [_i]),
     'odbox_set_nms_fused_tail': (_i, [_i]),
     'odbox_focal_loss_rows': (_i, [_vp, _vp, _sz, _i, _f, _f, _i, _vp, _vp, _vp]),
+    'odbox_label_logprobs_workspace': (_sz, [_sz, _i, _i]),
+    'odbox_label_logprobs': (_i, [_vp, _i, _sz, _i, _sz, _vp, _i, _f, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'odbox_label_logprobs_backward': (_i, [_vp, _i, _sz, _i, _sz, _vp, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _vp]),
+    'odbox_distill_loss_workspace': (_sz, [_sz, _i, _i]),
+    'odbox_distill_loss': (_i, [_vp, _i, _sz, _i, _sz, _vp, _vp, _i, _f, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'odbox_distill_loss_backward': (_i, [_vp, _i, _sz, _i, _sz, _vp, _vp, _i, _f, _i, _vp, _f, _vp, _vp, _i, _vp, _vp]),
     'odbox_bbox_overlap': (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _vp]),
     'odbox_bbox_transform': (_i, [_vp, _i, _vp, _i, _i, _vp, _vp]),
     'odbox_regress_boxes': (_i, [_vp, _i, _vp, _i, _i, _vp, _vp]),

@@ -27,6 +27,7 @@ UNITS = {
     'odbox_train.hip': os.environ.get('ODBOX_TRAIN_FLAGS', '').split(),
     'odbox_infer.hip': ['-fno-honor-nans'],
     'odbox_eval.hip': [],
+    'odbox_logits.hip': [],
 }
 HEADERS = [os.path.join(CSRC, 'odbox_common.h'), os.path.join(ROOT, 'include', 'odbox.h')]
 

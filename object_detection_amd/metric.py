@@ -8,9 +8,15 @@ pred_bboxes, pred_scores, pred_image_scores, training)` returns
 reference's running statistics in `train_metric` (`Metric`, metric.py:40-73): means of the losses
 and the two categorical accuracies, accumulated on the device without a host sync; the foreground
 accuracy's numerator comes out of the same kernel launch as the losses (out_loss[3]).
-HIP only (odbox_match_loss / odbox_focal_loss), no CPU fallback.
+`label_logprobs` and `distill_loss` work on rows of class logits beside `focal_loss(from_logits=True)`: scores of given
+labels with entropy and top alternatives, and distillation from a teacher's top classes (no counterpart in the reference).
+HIP only (odbox_match_loss / odbox_focal_loss / odbox_label_logprobs / odbox_distill_loss), no CPU fallback.
 """
+import contextlib
+import typing
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .anchors import _image_hw
@@ -114,6 +120,240 @@ def focal_loss(y_true, y_pred, gamma: float = 1.5, alpha: float = 0.25, from_log
     if return_grad:
         return loss, (grad * scale if scale != 1.0 else grad)
     return loss
+
+
+# ---- rows of class logits ----
+
+_DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}       # ODBOX_DTYPE_*
+MAX_TOP = 128                                                               # ODBOX_MAX_TOP
+MAX_LOGITS = 1 << 24                                                        # ODBOX_MAX_LOGITS
+_REST = {'renormalise': 0, 'bucket': 1}                                     # ODBOX_REST_*
+
+
+def _logits(x):
+    """Logits on their own GPU (host data: on the current one) in float32 / float16 / bfloat16; other types become float32."""
+    if not isinstance(x, torch.Tensor):
+        x = torch.as_tensor(x)
+    dev = x.device if x.is_cuda else _lib.require_gpu()
+    x = x.to(device=dev, dtype=x.dtype if x.dtype in _DTYPE_CODE else torch.float32, non_blocking=True)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_LOGITS:
+        raise ValueError('logits %r: the last axis holds 1..%d classes' % (tuple(x.shape), MAX_LOGITS))
+    return x
+
+
+def _rows_view(x):
+    """[..., C] -> ([rows, C] view, rows, C, elements between rows).  The classes of a row have to lie side by side and the
+    rows evenly apart (a padded vocabulary, an expanded row): anything else is copied once."""
+    C = int(x.shape[-1])
+    rows = x.numel() // C
+    if rows == 0:
+        return x.reshape(0, C), 0, C, C
+    if x.dim() == 1:
+        x = x.unsqueeze(0)
+    if C > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    try:
+        v = x.view(rows, C)
+    except RuntimeError:
+        v = x.contiguous().view(rows, C)
+    return v, rows, C, (int(v.stride(0)) if rows > 1 else C)
+
+
+def _side(x, dtype, device, shape, what):
+    """A tensor that goes with the rows of the logits, contiguous on their device."""
+    if not isinstance(x, torch.Tensor):
+        x = torch.as_tensor(x)
+    if tuple(x.shape) != tuple(shape):
+        raise ValueError('%s %r does not fit the logits: expected %r' % (what, tuple(x.shape), tuple(shape)))
+    return x.detach().to(device=device, dtype=dtype, non_blocking=True).contiguous()
+
+
+def _temperature(t):
+    t = float(t)
+    if not 1e-6 <= t <= 1e6:
+        raise ValueError('temperature %r is not in 1e-6..1e6' % t)
+    return t
+
+
+def _on(device):
+    """Launches go to the logits' device and its current stream, whichever device is current."""
+    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+class LabelLogprobs(typing.NamedTuple):
+    """What `label_logprobs` returns; fields that were not asked for are None."""
+    logprobs: typing.Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_logprobs: typing.Optional[torch.Tensor]
+    top_labels: typing.Optional[torch.Tensor]
+
+
+def _score_launch(x, labels, top_k, temperature, want_stats):
+    lib = _lib.load()
+    v, rows, C, stride = _rows_view(x)
+    lead = x.shape[:-1]
+    new = dict(dtype=torch.float32, device=x.device)
+    ent = torch.empty(lead, **new)
+    lp = torch.empty(lead, **new) if labels is not None else None
+    tlp = torch.empty(lead + (top_k,), **new) if top_k else None
+    tid = torch.empty(lead + (top_k,), dtype=torch.int32, device=x.device) if top_k else None
+    stats = torch.empty((rows, 4), **new) if want_stats else None
+    need = lib.odbox_label_logprobs_workspace(rows, C, top_k)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _lib.check(lib.odbox_label_logprobs(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _lib.ptr(labels), top_k, temperature,
+                                        _lib.ptr(lp), _lib.ptr(ent), _lib.ptr(tlp), _lib.ptr(tid), _lib.ptr(stats),
+                                        _lib.ptr(ws), need, _lib.stream_ptr()), 'odbox_label_logprobs')
+    return lp, ent, tlp, tid, stats
+
+
+def _upstream(g, device):
+    return None if g is None else g.detach().to(device=device, dtype=torch.float32).contiguous()
+
+
+class _LabelLogprobsFn(torch.autograd.Function):
+    """The forward launch keeps four floats a row; the backward launch reads the logits again and writes the gradient once."""
+
+    @staticmethod
+    def forward(ctx, x, labels, top_k, temperature):
+        ctx.set_materialize_grads(False)
+        with _on(x.device):
+            lp, ent, tlp, tid, stats = _score_launch(x, labels, top_k, temperature, True)
+        ctx.save_for_backward(x, labels, tid, stats)
+        ctx.cfg = (top_k, temperature)
+        if tid is not None:
+            ctx.mark_non_differentiable(tid)
+        return lp, ent, tlp, tid
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _g_id):
+        x, labels, tid, stats = ctx.saved_tensors
+        top_k, temperature = ctx.cfg
+        if g_lp is None and g_ent is None and g_top is None:
+            return None, None, None, None
+        lib = _lib.load()
+        with _on(x.device):
+            v, rows, C, stride = _rows_view(x)
+            g_lp, g_ent, g_top = (_upstream(g, x.device) for g in (g_lp, g_ent, g_top))
+            grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            _lib.check(lib.odbox_label_logprobs_backward(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _lib.ptr(labels), top_k,
+                                                         _lib.ptr(tid), temperature, _lib.ptr(stats), _lib.ptr(g_lp), _lib.ptr(g_ent),
+                                                         _lib.ptr(g_top), _lib.ptr(grad), _lib.stream_ptr()),
+                       'odbox_label_logprobs_backward')
+        return grad, None, None, None
+
+
+def label_logprobs(logits, labels=None, top_k: int = 0, temperature: float = 1.0) -> LabelLogprobs:
+    """Scores of rows of class logits [..., C] (float32, float16, bfloat16) under softmax(logits / temperature), in one pass:
+
+    logprobs [...]          log-probability of labels [...] (int; a label outside [0, C) marks a padded row: 0, no gradient);
+                            None without labels
+    entropy [...]           -sum p log p, in nats
+    top_logprobs [..., k],  the top_k (<= 128) classes of largest logit and their log-probabilities, largest first, ties to
+    top_labels [..., k]     the lowest class (int32); None when top_k is 0
+
+    All results are float32.  Rows may lie apart (logits[:, :C] of a padded class axis is read in place).  Differentiable
+    w.r.t. the logits through logprobs, entropy and top_logprobs (odbox_label_logprobs_backward; the gradient has the logits'
+    type).  A logit of -inf is a forbidden class; a row of nothing else gives log-probabilities -inf, entropy 0 and no
+    gradient; a NaN or +inf makes its row NaN.  On a teacher, `top_logprobs` / `top_labels` are what `distill_loss` takes."""
+    x = _logits(logits)
+    temperature = _temperature(temperature)
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(MAX_TOP, x.shape[-1]):
+        raise ValueError('top_k %d is not in 0..min(%d classes, %d)' % (top_k, x.shape[-1], MAX_TOP))
+    if labels is not None:
+        labels = _side(labels, torch.int32, x.device, x.shape[:-1], 'labels')
+    if torch.is_grad_enabled() and x.requires_grad:
+        return LabelLogprobs(*_LabelLogprobsFn.apply(x, labels, top_k, temperature))
+    with _on(x.device):
+        return LabelLogprobs(*_score_launch(x.detach(), labels, top_k, temperature, False)[:4])
+
+
+def _distill_launch(x, tl, ids, w, cfg, per_row, want_stats, want_grad):
+    lib = _lib.load()
+    temperature, rest, scale = cfg
+    v, rows, C, stride = _rows_view(x)
+    K = int(ids.shape[-1])
+    new = dict(dtype=torch.float32, device=x.device)
+    out = torch.empty(x.shape[:-1] if per_row else (), **new)
+    stats = torch.empty((rows, 4), **new) if want_stats else None
+    grad = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_grad else None
+    need = lib.odbox_distill_loss_workspace(rows, C, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _lib.check(lib.odbox_distill_loss(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _lib.ptr(tl), _lib.ptr(ids), K, temperature,
+                                      rest, _lib.ptr(w), scale, _lib.ptr(out) if per_row else None,
+                                      None if per_row else _lib.ptr(out), _lib.ptr(stats), _lib.ptr(grad), _lib.ptr(ws), need,
+                                      _lib.stream_ptr()), 'odbox_distill_loss')
+    return out, stats, grad
+
+
+class _DistillLossFn(torch.autograd.Function):
+    """The forward launch keeps four floats a row; the backward launch reads the logits again and writes the gradient once,
+    with the upstream value read on the device."""
+
+    @staticmethod
+    def forward(ctx, x, tl, ids, w, cfg, per_row):
+        with _on(x.device):
+            out, stats, _ = _distill_launch(x, tl, ids, w, cfg, per_row, True, False)
+        ctx.save_for_backward(x, tl, ids, w, stats)
+        ctx.cfg, ctx.per_row = cfg, per_row
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, tl, ids, w, stats = ctx.saved_tensors
+        temperature, rest, scale = ctx.cfg
+        lib = _lib.load()
+        with _on(x.device):
+            v, rows, C, stride = _rows_view(x)
+            g = _upstream(g, x.device)
+            grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            _lib.check(lib.odbox_distill_loss_backward(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _lib.ptr(tl), _lib.ptr(ids),
+                                                       int(ids.shape[-1]), temperature, rest, _lib.ptr(w), scale, _lib.ptr(stats),
+                                                       _lib.ptr(g), int(ctx.per_row), _lib.ptr(grad), _lib.stream_ptr()),
+                       'odbox_distill_loss_backward')
+        return grad, None, None, None, None, None
+
+
+def distill_loss(logits, teacher_logprobs, teacher_labels, temperature: float = 1.0, rest: str = 'renormalise', row_weights=None,
+                 reduction: str = 'sum', return_grad: bool = False):
+    """Distillation of a student's class logits [..., C] from the K (<= 128) classes a teacher ranks best:
+    teacher_labels [..., K] their ids (an id outside [0, C) is an unused place), teacher_logprobs [..., K] their
+    log-probabilities at the same temperature T, as `label_logprobs(teacher, top_k=K, temperature=T)` returns them.
+    With q the teacher's probabilities, p = softmax(logits / T) and w = row_weights [...] (default 1)
+
+        loss[row] = w T^2 [ sum_k q_k (log q_k - log p[id_k]) + rest ]
+
+    rest='renormalise': q is renormalised over the list and rest is 0 (a common shift of the teacher's values cancels, so the
+    teacher's logits / T will do).  rest='bucket': q is taken as it is and all classes off the list form one more class,
+    rest = q0 (log q0 - log p0).  A row of weight 0 is ignored whatever it holds.
+
+    reduction 'sum' (default), 'mean' (over the rows; 0 for none) or anything else (e.g. None): the losses [...] themselves,
+    float32.  Differentiable w.r.t. the logits; return_grad=True instead returns (loss, gradient), the gradient in the
+    logits' type from the same call -- one pass over the logits where autograd takes two -- of the reduced loss, or for
+    un-reduced losses of each row's loss w.r.t. that row."""
+    x = _logits(logits)
+    temperature = _temperature(temperature)
+    if rest not in _REST:
+        raise ValueError("rest %r is neither 'renormalise' nor 'bucket'" % (rest,))
+    if not isinstance(teacher_labels, torch.Tensor):
+        teacher_labels = torch.as_tensor(teacher_labels)
+    lead = tuple(x.shape[:-1])
+    K = int(teacher_labels.shape[-1]) if teacher_labels.dim() else 0
+    if not 1 <= K <= MAX_TOP:
+        raise ValueError('teacher_labels %r: the last axis holds 1..%d classes' % (tuple(teacher_labels.shape), MAX_TOP))
+    ids = _side(teacher_labels, torch.int32, x.device, lead + (K,), 'teacher_labels')
+    tl = _side(teacher_logprobs, torch.float32, x.device, lead + (K,), 'teacher_logprobs')
+    w = None if row_weights is None else _side(row_weights, torch.float32, x.device, lead, 'row_weights')
+    per_row = reduction not in ('sum', 'mean')
+    rows = x.numel() // x.shape[-1]
+    cfg = (temperature, _REST[rest], 1.0 / max(rows, 1) if reduction == 'mean' else 1.0)
+    if not return_grad and torch.is_grad_enabled() and x.requires_grad:
+        return _DistillLossFn.apply(x, tl, ids, w, cfg, per_row)
+    with _on(x.device):
+        loss, _, grad = _distill_launch(x.detach(), tl, ids, w, cfg, per_row, False, return_grad)
+    return (loss, grad) if return_grad else loss
 
 
 def _pred_dtype(pred_bboxes, pred_scores):
