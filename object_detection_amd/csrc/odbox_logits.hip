@@ -13,61 +13,156 @@ namespace odbox {
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
 constexpr float T_FLOOR = -16384.0f;             // stands for log2 p = -inf in p * log2 p (2^-16384 is 0, so the product is 0)
-constexpr int LG_THREADS = 256;
-constexpr int LG_WAVES = LG_THREADS / WAVE;
+constexpr float M_START = -1e30f;                // a running maximum before any class; times c it is still finite
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Element types: 16-byte vectors that may start at any element (rows of an odd number of classes do: global_load / store_dwordx4
+// take any alignment).  Stores round to nearest even.
+template <class V, int ALIGN>
+struct Unaligned {
+    typedef V type __attribute__((aligned(ALIGN)));
+};
 struct F32 {
     using raw = float;
+    static constexpr int VEC = 4;
     static __device__ __forceinline__ float get(raw v) { return v; }
     static __device__ __forceinline__ raw put(float v) { return v; }
+    static __device__ __forceinline__ void unpack(u32x4 w, float *v)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+    }
+    static __device__ __forceinline__ u32x4 pack(const float *v)
+    {
+        return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    }
 };
 struct F16 {
     using raw = _Float16;
+    static constexpr int VEC = 8;
     static __device__ __forceinline__ float get(raw v) { return (float)v; }
     static __device__ __forceinline__ raw put(float v) { return (_Float16)v; }
+    static __device__ __forceinline__ void unpack(u32x4 w, float *v)
+    {
+        const f16x8 h = __builtin_bit_cast(f16x8, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+    }
+    static __device__ __forceinline__ u32x4 pack(const float *v)
+    {
+        f16x8 h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i];
+        return __builtin_bit_cast(u32x4, h);
+    }
 };
 struct BF16 {
     using raw = uint16_t;
+    static constexpr int VEC = 8;
     static __device__ __forceinline__ float get(raw v) { return __uint_as_float((uint32_t)v << 16); }
-    // round to nearest even; a NaN keeps its sign and becomes quiet (the carry of the rounding must not turn it into inf)
-    static __device__ __forceinline__ raw put(float v)
+    static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(raw, (__bf16)v); }
+    static __device__ __forceinline__ void unpack(u32x4 w, float *v)
     {
-        const uint32_t u = __float_as_uint(v);
-        if ((u & 0x7fffffffu) > 0x7f800000u) return (raw)((u >> 16) | 0x40u);
-        return (raw)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float *v)
+    {
+        f32x8 f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = v[i];
+        return __builtin_bit_cast(u32x4, __builtin_convertvector(f, bf16x8));
     }
 };
+template <class E>
+__device__ __forceinline__ u32x4 load_raw(const typename E::raw *p)
+{
+    typedef typename Unaligned<u32x4, sizeof(typename E::raw)>::type mem;
+    return *(const mem *)p;
+}
+template <class E>
+__device__ __forceinline__ void store_raw(typename E::raw *p, u32x4 v)
+{
+    typedef typename Unaligned<u32x4, sizeof(typename E::raw)>::type mem;
+    *(mem *)p = v;
+}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float vmax3(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
-// What one block shares: wave partials of the reductions, the radix histogram, the chosen keys.
+// ------------------------------------------------------------------------------------------
+// reductions over a wave (DPP) and a block
+// ------------------------------------------------------------------------------------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_f(float old, float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(x), CTRL, ROWS, 0xf, false));
+}
+// x of the wave's lanes combined in lane 63 and handed to all; `none` is the operation's neutral value
+template <class Op>
+__device__ __forceinline__ float wave_reduce(float x, float none, Op op)
+{
+    x = op(x, dpp_f<0x111, 0xf>(none, x));       // row_shr:1
+    x = op(x, dpp_f<0x112, 0xf>(none, x));       // row_shr:2
+    x = op(x, dpp_f<0x114, 0xf>(none, x));       // row_shr:4
+    x = op(x, dpp_f<0x118, 0xf>(none, x));       // row_shr:8
+    x = op(x, dpp_f<0x142, 0xa>(none, x));       // row_bcast:15 into rows 1 and 3
+    x = op(x, dpp_f<0x143, 0xc>(none, x));       // row_bcast:31 into rows 2 and 3
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+__device__ __forceinline__ float wave_max(float x) { return wave_reduce(x, -INFINITY, [](float a, float b) { return vmax(a, b); }); }
+__device__ __forceinline__ float wave_sum(float x) { return wave_reduce(x, 0.0f, [](float a, float b) { return a + b; }); }
+
+constexpr uint32_t TOP_CAP = 1024;               // candidates of a row's top classes
+constexpr uint32_t MAX_WAVES = 16;
+constexpr uint32_t LIST_MAX = ODBOX_MAX_TOP + 1;
+
+// What one block shares.
 struct LogitsLds {
-    double d[LG_WAVES];
-    float f[LG_WAVES];
-    uint32_t hist[256];
-    uint64_t key[ODBOX_MAX_TOP];
+    double d[MAX_WAVES];
+    float f[MAX_WAVES];
+    float3 part[MAX_WAVES];
     uint32_t count;
     uint32_t pick[2];
-    int32_t id[ODBOX_MAX_TOP + 1];
-    float val[ODBOX_MAX_TOP + 1];
+    int32_t id[LIST_MAX];
+    float val[LIST_MAX];
+};
+struct TopLds {
+    uint32_t group[256];                         // group maxima of the selection; the radix histogram
+    uint64_t key[TOP_CAP];
 };
 
-template <class Op>
-__device__ __forceinline__ float block_reduce(float v, LogitsLds &sh, Op op)
+template <int NT, class Op>
+__device__ __forceinline__ float block_reduce(float v, float none, LogitsLds &sh, Op op)
 {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = op(v, __shfl_xor(v, off));
+    v = wave_reduce(v, none, op);
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) sh.f[threadIdx.x >> 6] = v;
     __syncthreads();
     v = sh.f[0];
 #pragma unroll
-    for (int w = 1; w < LG_WAVES; ++w) v = op(v, sh.f[w]);
+    for (int w = 1; w < NT / WAVE; ++w) v = op(v, sh.f[w]);
     return v;
 }
-__device__ __forceinline__ float block_max(float v, LogitsLds &sh) { return block_reduce(v, sh, [](float a, float b) { return vmax(a, b); }); }
-__device__ __forceinline__ float block_sum(float v, LogitsLds &sh) { return block_reduce(v, sh, [](float a, float b) { return a + b; }); }
+template <int NT>
+__device__ __forceinline__ float block_max(float v, LogitsLds &sh) { return block_reduce<NT>(v, -INFINITY, sh, [](float a, float b) { return vmax(a, b); }); }
+template <int NT>
+__device__ __forceinline__ float block_sum(float v, LogitsLds &sh) { return block_reduce<NT>(v, 0.0f, sh, [](float a, float b) { return a + b; }); }
+template <int NT>
 __device__ __forceinline__ double block_sum_f64(double v, LogitsLds &sh)
 {
 #pragma unroll
@@ -77,44 +172,165 @@ __device__ __forceinline__ double block_sum_f64(double v, LogitsLds &sh)
     __syncthreads();
     v = sh.d[0];
 #pragma unroll
-    for (int w = 1; w < LG_WAVES; ++w) v += sh.d[w];
+    for (int w = 1; w < NT / WAVE; ++w) v += sh.d[w];
     return v;
 }
 
+// ------------------------------------------------------------------------------------------
+// softmax statistics of a row
+// ------------------------------------------------------------------------------------------
 struct RowStats {
     float m;             // largest logit; -inf: every logit is -inf (an empty row); NaN: the row holds a NaN or +inf
     float l2;            // log2 of the sum
     float ent;           // entropy in nats
 };
 
-// Two passes over the row by the whole block.  skip(i): class i is left out.
-template <class E, class Skip>
-__device__ RowStats row_stats(const typename E::raw *x, uint32_t C, float c, LogitsLds &sh, Skip skip)
+// One thread's share of a row in one pass: maximum m, s = sum 2^(x c - mc) and u = sum 2^(x c - mc) (x c - mc), mc = m c as
+// rounded (nmc = -mc).  The fused multiply-add rounds x c - mc once, and join() takes the rounding of mc out again.
+struct Running {
+    float m, nmc, s, u;
+};
+__device__ __forceinline__ Running running_start(float c) { return {M_START, -(M_START * c), 0.0f, 0.0f}; }
+
+// N values at once: one maximum, one rescaling.  A class at -inf adds 0; what a NaN, an infinity or values whose product with c
+// overflows do to s, row_ok() sees.
+template <int N, bool ENT>
+__device__ __forceinline__ void absorb(const float *v, float c, Running &r)
+{
+    float g = r.m;
+    if (N == 1) g = vmax(g, v[0]);
+#pragma unroll
+    for (int i = 0; i + 1 < N; i += 2) g = vmax3(g, v[i], v[i + 1]);
+    const float nmc = -(g * c), d = nmc - r.nmc, f = exp2_hw(d);
+    if (ENT) r.u = __builtin_fmaf(d, r.s, r.u) * f;
+    r.s *= f;
+    r.m = g;
+    r.nmc = nmc;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = __builtin_fmaf(v[i], c, nmc), e = exp2_hw(t);
+        s += e;
+        if (ENT) r.u = __builtin_fmaf(e, vmax(t, T_FLOOR), r.u);
+    }
+    r.s += s;
+}
+
+// Shares of a wave, then of a block, about the common maximum M: x -> float3(M, sum 2^((x - M) c), sum of the same times its exponent)
+__device__ __forceinline__ float3 wave_join(const Running &r, float c)
+{
+    const float M = wave_max(r.m);
+    const float D = (r.m - M) * c + __builtin_fmaf(-r.m, c, -r.nmc), f = exp2_hw(D);
+    const bool some = r.s != 0.0f;               // (a share without classes would make 0 * inf out of its M_START)
+    return make_float3(M, wave_sum(some ? r.s * f : 0.0f), wave_sum(some ? __builtin_fmaf(D, r.s, r.u) * f : 0.0f));
+}
+__device__ __forceinline__ float3 join(const float3 *part, uint32_t n, float c)
+{
+    float M = part[0].x;
+    for (uint32_t w = 1; w < n; ++w) M = vmax(M, part[w].x);
+    float s = 0.0f, u = 0.0f;
+    for (uint32_t w = 0; w < n; ++w) {
+        const float3 p = part[w];
+        const float D = (p.x - M) * c, f = exp2_hw(D);
+        if (p.y != 0.0f) s += p.y * f, u += __builtin_fmaf(D, p.y, p.z) * f;
+    }
+    return make_float3(M, s, u);
+}
+template <int NT>
+__device__ __forceinline__ float3 block_join(const Running &r, float c, LogitsLds &sh)
+{
+    const float3 p = wave_join(r, c);
+    __syncthreads();
+    if ((threadIdx.x & 63u) == 0) sh.part[threadIdx.x >> 6] = p;
+    __syncthreads();
+    return join(sh.part, NT / WAVE, c);
+}
+// Whether one pass sufficed.  Not so where no class lies above M_START (all forbidden, all at the type's lowest value) or
+// where a NaN, an infinity or an overflow of m c made the sum 0, infinite or NaN.
+__device__ __forceinline__ bool row_ok(const float3 &j) { return j.y > 0.0f && j.y < INFINITY; }
+__device__ __forceinline__ RowStats stats_of(const float3 &j)
+{
+    const float l2 = log2_hw(j.y);
+    return {j.x, l2, LN2 * (l2 - j.z / j.y)};
+}
+
+// Two passes over the row by the whole block, for the rows that are not row_ok.  skip(i): class i is left out.
+template <class E, int NT, class Skip>
+__device__ __attribute__((noinline)) RowStats careful_stats(const typename E::raw *x, uint32_t C, float c, LogitsLds &sh, Skip skip)
 {
     float m = -INFINITY, bad = 0.0f;
-    for (uint32_t i = threadIdx.x; i < C; i += LG_THREADS) {
+    for (uint32_t i = threadIdx.x; i < C; i += NT) {
         const float v = E::get(x[i]);
         if (skip(i)) continue;
         if (v != v || v == INFINITY) bad = 1.0f;
         m = vmax(m, v);
     }
-    m = block_max(m, sh);
-    bad = block_max(bad, sh);
+    m = block_max<NT>(m, sh);
+    bad = block_max<NT>(bad, sh);
     if (bad != 0.0f) return {NAN, NAN, NAN};
     if (m == -INFINITY) return {m, -INFINITY, 0.0f};
     float s = 0.0f, u = 0.0f;
-    for (uint32_t i = threadIdx.x; i < C; i += LG_THREADS) {
+    for (uint32_t i = threadIdx.x; i < C; i += NT) {
         if (skip(i)) continue;
         const float t = (E::get(x[i]) - m) * c, e = exp2_hw(t);
         s += e;
         u += e * vmax(t, T_FLOOR);
     }
-    s = block_sum(s, sh);
-    u = block_sum(u, sh);
+    s = block_sum<NT>(s, sh);
+    u = block_sum<NT>(u, sh);
     const float l2 = log2_hw(s);
     return {m, l2, LN2 * (l2 - u / s)};
 }
 
+// A block's pass over n classes.  MASK: bit e of mask[v] leaves element e of vector v out.
+template <class E, int NT, int U, bool ENT, bool MASK>
+__device__ __forceinline__ Running scan_classes(const typename E::raw *x, uint32_t n, float c, const uint8_t *mask)
+{
+    constexpr int VEC = E::VEC;
+    const uint32_t nvec = n / VEC;
+    Running r = running_start(c);
+    uint32_t i = threadIdx.x;
+    for (; i + (U - 1) * NT < nvec; i += U * NT) {
+        u32x4 w[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) w[k] = load_raw<E>(x + (size_t)(i + k * NT) * VEC);
+        float v[U * VEC];
+#pragma unroll
+        for (int k = 0; k < U; ++k) E::unpack(w[k], v + k * VEC);
+        if (MASK) {
+            uint32_t b[U], any = 0;
+#pragma unroll
+            for (int k = 0; k < U; ++k) any |= b[k] = mask[i + k * NT];
+            if (__any(any)) {
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) v[k * VEC + e] = b[k] >> e & 1u ? -INFINITY : v[k * VEC + e];
+            }
+        }
+        absorb<U * VEC, ENT>(v, c, r);
+    }
+    for (; i < nvec; i += NT) {
+        float v[VEC];
+        E::unpack(load_raw<E>(x + (size_t)i * VEC), v);
+        if (MASK) {
+            const uint32_t b = mask[i];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = b >> e & 1u ? -INFINITY : v[e];
+        }
+        absorb<VEC, ENT>(v, c, r);
+    }
+    if (threadIdx.x < n - nvec * VEC) {
+        float v = E::get(x[nvec * VEC + threadIdx.x]);
+        if (MASK) v = mask[nvec] >> threadIdx.x & 1u ? -INFINITY : v;
+        absorb<1, ENT>(&v, c, r);
+    }
+    return r;
+}
+
+// ------------------------------------------------------------------------------------------
+// top classes
+// ------------------------------------------------------------------------------------------
 // Order of the top alternatives: value descending, then index ascending; NaN above everything.  56 significant bits.
 __device__ __forceinline__ uint64_t top_key(float v, uint32_t i)
 {
@@ -122,26 +338,44 @@ __device__ __forceinline__ uint64_t top_key(float v, uint32_t i)
     return ((uint64_t)o << 24) | (0xffffffu - i);
 }
 __device__ __forceinline__ uint32_t top_index(uint64_t k) { return 0xffffffu - ((uint32_t)k & 0xffffffu); }
+__device__ __forceinline__ float top_value(uint64_t k)
+{
+    const uint32_t o = (uint32_t)(k >> 24);
+    return o == 0xffffffffu ? NAN : f32_unordered(o);
+}
 
-// The k (<= ODBOX_MAX_TOP, <= n) largest of n unique keys into sh.key, ordered descending: the k-th key by a radix selection of
-// eight bits a pass, then exactly k keys are collected and each counts those above it.
-template <class Key>
-__device__ void top_radix(uint32_t n, uint32_t k, LogitsLds &sh, Key key)
+// n candidates in top.key, unordered, the k largest of the whole among them: each counts the larger ones, out(rank, key) is
+// called for the first k.
+template <int NT, class Out>
+__device__ __forceinline__ void rank_candidates(uint32_t n, uint32_t k, const TopLds &top, Out out)
+{
+    for (uint32_t t = threadIdx.x; t < n; t += NT) {
+        const uint64_t mine = top.key[t];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; ++j) rank += top.key[j] > mine;
+        if (rank < k) out(rank, mine);
+    }
+}
+
+// The k (<= ODBOX_MAX_TOP, <= n) largest of n unique keys: the k-th key by a radix selection of eight bits a pass, then exactly k
+// keys are collected.  Right for every input, eight passes: where the threshold below keeps too few or too many candidates.
+template <int NT, class Key, class Out>
+__device__ __attribute__((noinline)) void top_radix(uint32_t n, uint32_t k, LogitsLds &sh, TopLds &top, Key key, Out out)
 {
     uint64_t prefix = 0;
     uint32_t want = k;
     for (int shift = 48; shift >= 0; shift -= 8) {
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < 256; i += LG_THREADS) sh.hist[i] = 0;
+        for (uint32_t i = threadIdx.x; i < 256; i += NT) top.group[i] = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += LG_THREADS) {
+        for (uint32_t i = threadIdx.x; i < n; i += NT) {
             const uint64_t q = key(i);
-            if ((q >> shift >> 8) == prefix) atomicAdd(&sh.hist[(uint32_t)(q >> shift) & 255u], 1u);
+            if ((q >> shift >> 8) == prefix) atomicAdd(&top.group[(uint32_t)(q >> shift) & 255u], 1u);
         }
         __syncthreads();
         if (threadIdx.x == 0) {
             uint32_t above = 0, b = 255;
-            while (b > 0 && above + sh.hist[b] < want) above += sh.hist[b--];
+            while (b > 0 && above + top.group[b] < want) above += top.group[b--];
             sh.pick[0] = b;
             sh.pick[1] = above;
         }
@@ -152,22 +386,107 @@ __device__ void top_radix(uint32_t n, uint32_t k, LogitsLds &sh, Key key)
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    uint64_t mine = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += LG_THREADS) {
+    for (uint32_t i = threadIdx.x; i < n; i += NT) {
         const uint64_t q = key(i);
-        if (q >= prefix) sh.key[atomicAdd(&sh.count, 1u)] = q;        // unique keys: exactly k of them
+        if (q >= prefix) top.key[atomicAdd(&sh.count, 1u)] = q;       // unique keys: exactly k of them
     }
     __syncthreads();
-    uint32_t rank = 0;
-    if (threadIdx.x < k) {
-        mine = sh.key[threadIdx.x];
-        for (uint32_t j = 0; j < k; ++j) rank += sh.key[j] > mine;
-    }
-    __syncthreads();
-    if (threadIdx.x < k) sh.key[rank] = mine;
+    rank_candidates<NT>(k, k, top, out);
     __syncthreads();
 }
 
+// A value (in f32_ordered form) that at least k of the row's classes reach and few more do: the k-th largest of 64 or 256 group
+// maxima, a group being the classes of NT / 64 or NT / 256 neighbouring threads (>= 2 k groups keep about 1.4 k candidates of
+// values in no particular order).  mine: the thread's largest value.
+template <int NT>
+__device__ __forceinline__ uint32_t top_threshold(uint32_t mine, uint32_t k, LogitsLds &sh, TopLds &top)
+{
+    auto fold = [&](int lanes) {
+        uint32_t v = mine;
+        for (int off = 1; off < lanes; off <<= 1) {
+            const uint32_t o = __shfl_xor(v, off);
+            v = o > v ? o : v;
+        }
+        return v;
+    };
+    const uint32_t G = k <= 32 ? 64 : 256;
+    const uint32_t lanes = NT / G;
+    const uint32_t v = fold((int)lanes);
+    __syncthreads();
+    if (threadIdx.x % lanes == 0) top.group[threadIdx.x / lanes] = v;
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    if (threadIdx.x < G) {
+        const uint32_t w = top.group[threadIdx.x];
+        uint32_t gt = 0, ge = 0;
+        for (uint32_t j = 0; j < G; j += 4) {
+            const uint4 q = *(const uint4 *)&top.group[j];
+            gt += (q.x > w) + (q.y > w) + (q.z > w) + (q.w > w);
+            ge += (q.x >= w) + (q.y >= w) + (q.z >= w) + (q.w >= w);
+        }
+        if (gt < k && k <= ge) sh.pick[0] = w;   // one value, whoever writes it
+    }
+    __syncthreads();
+    return sh.pick[0];
+}
+__device__ __forceinline__ void push_candidate(uint64_t key, LogitsLds &sh, TopLds &top)
+{
+    const uint32_t at = atomicAdd(&sh.count, 1u);
+    if (at < TOP_CAP) top.key[at] = key;
+}
+
+// The k best of the n classes at x, whose indices start at first.  m: the thread's largest value in scan_classes' order of work, so
+// only threads that hold a candidate look at their classes again.
+template <class E, int NT, int U, class Out>
+__device__ __forceinline__ void top_classes(const typename E::raw *x, uint32_t n, uint32_t first, uint32_t k, float m, bool ok, LogitsLds &sh,
+                                            TopLds &top, Out out)
+{
+    constexpr int VEC = E::VEC;
+    bool few = false;
+    if (ok) {
+        const uint32_t tau = top_threshold<NT>(f32_ordered(m), k, sh, top);
+        const float floor_ = f32_unordered(tau);
+        if (m >= floor_) {
+            const uint32_t nvec = n / VEC;
+            uint32_t i = threadIdx.x;
+            auto look = [&](float v, uint32_t at) {
+                if (v >= floor_) push_candidate(top_key(v, first + at), sh, top);
+            };
+            for (; i + (U - 1) * NT < nvec; i += U * NT) {
+                u32x4 w[U];
+#pragma unroll
+                for (int j = 0; j < U; ++j) w[j] = load_raw<E>(x + (size_t)(i + j * NT) * VEC);
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    float v[VEC], g = -INFINITY;
+                    E::unpack(w[j], v);
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 2) g = vmax3(g, v[e], v[e + 1]);
+                    if (g >= floor_)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) look(v[e], (i + j * NT) * VEC + e);
+                }
+            }
+            for (; i < nvec; i += NT) {
+                float v[VEC];
+                E::unpack(load_raw<E>(x + (size_t)i * VEC), v);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) look(v[e], i * VEC + e);
+            }
+            if (threadIdx.x < n - nvec * VEC) look(E::get(x[nvec * VEC + threadIdx.x]), nvec * VEC + threadIdx.x);
+        }
+        __syncthreads();
+        const uint32_t got = sh.count;
+        few = got >= k && got <= TOP_CAP;
+        if (few) rank_candidates<NT>(got, k, top, out);
+        __syncthreads();
+    }
+    if (!few) top_radix<NT>(n, k, sh, top, [&](uint32_t i) { return top_key(E::get(x[i]), first + i); }, out);
+}
+
+// ------------------------------------------------------------------------------------------
+// scores
+// ------------------------------------------------------------------------------------------
 struct ScoreArgs {
     const void *logits;
     size_t rows, stride;
@@ -177,52 +496,131 @@ struct ScoreArgs {
     float *logprobs, *entropy, *top_logprobs;
     int32_t *top_labels;
     float4 *stats;
+    uint32_t segs, seg;                          // a row's classes go to `segs` blocks, `seg` (a multiple of 8) to each
+    float4 *part;                                // [rows, segs] shares of a split row
+    uint64_t *part_key;                          // [rows, segs, k]
 };
 
 template <class E>
-__global__ __launch_bounds__(LG_THREADS) void score_rows_kernel(ScoreArgs a)
+__device__ __forceinline__ float logprob_of(const ScoreArgs &a, const RowStats &st, float v)
 {
+    return st.m == -INFINITY ? -INFINITY : (v - st.m) * a.inv_t - LN2 * st.l2;
+}
+template <class E>
+__device__ __forceinline__ void score_out(const ScoreArgs &a, size_t row, const typename E::raw *x, const RowStats &st)
+{
+    if (threadIdx.x != 0) return;
+    if (a.logprobs) {
+        const uint32_t lab = (uint32_t)a.labels[row];
+        a.logprobs[row] = lab < a.C ? logprob_of<E>(a, st, E::get(x[lab])) : 0.0f;
+    }
+    if (a.entropy) a.entropy[row] = st.ent;
+    if (a.stats) a.stats[row] = make_float4(st.m, st.l2, st.ent, 0.0f);
+}
+
+// One block per row or per segment of a row.
+template <class E, int NT, bool TOP>
+__global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a)
+{
+    constexpr int U = 32 / E::VEC;               // 64 (float32: 128) bytes of loads in flight per thread
     __shared__ LogitsLds sh;
+    __shared__ TopLds top;
+    const size_t work = a.rows * a.segs;
+    for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
+        const size_t row = a.segs == 1 ? w : w / a.segs;
+        const uint32_t seg = a.segs == 1 ? 0 : (uint32_t)(w - row * a.segs), first = seg * a.seg;
+        const uint32_t n = a.C - first < a.seg ? a.C - first : a.seg;
+        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
+        const Running r = scan_classes<E, NT, U, true, false>(x + first, n, a.c, nullptr);
+        const float3 j = block_join<NT>(r, a.c, sh);
+        const bool ok = row_ok(j);
+        if (a.segs > 1) {
+            if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, j.z, 0.0f);
+            if (TOP) {
+                const uint32_t k = a.k < n ? a.k : n;        // a short last segment fills up with keys below every class's
+                for (uint32_t t = k + threadIdx.x; t < a.k; t += NT) a.part_key[w * a.k + t] = 0;
+                top_classes<E, NT, U>(x + first, n, first, k, r.m, ok, sh, top, [&](uint32_t rank, uint64_t key) { a.part_key[w * a.k + rank] = key; });
+            }
+            continue;
+        }
+        const RowStats st = ok ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, sh, [](uint32_t) { return false; });
+        score_out<E>(a, row, x, st);
+        if (TOP) top_classes<E, NT, U>(x, n, 0, a.k, r.m, ok, sh, top, [&](uint32_t rank, uint64_t key) {
+            a.top_labels[row * a.k + rank] = (int32_t)top_index(key);
+            a.top_logprobs[row * a.k + rank] = logprob_of<E>(a, st, top_value(key));
+        });
+    }
+}
+
+// The shares of a split row put together, one block a row.
+constexpr int JOIN_THREADS = 256;
+template <class E>
+__global__ __launch_bounds__(JOIN_THREADS) void score_join_kernel(ScoreArgs a)
+{
+    constexpr int NT = JOIN_THREADS;
+    __shared__ LogitsLds sh;
+    __shared__ TopLds top;
     for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        const RowStats st = row_stats<E>(x, a.C, a.c, sh, [](uint32_t) { return false; });
-        auto logprob = [&](float v) { return st.m == -INFINITY ? -INFINITY : (v - st.m) * a.inv_t - LN2 * st.l2; };
-        if (threadIdx.x == 0) {
-            if (a.logprobs) {
-                const uint32_t lab = (uint32_t)a.labels[row];
-                a.logprobs[row] = lab < a.C ? logprob(E::get(x[lab])) : 0.0f;
-            }
-            if (a.entropy) a.entropy[row] = st.ent;
-            if (a.stats) a.stats[row] = make_float4(st.m, st.l2, st.ent, 0.0f);
+        Running r = running_start(a.c);
+        for (uint32_t i = threadIdx.x; i < a.segs; i += NT) {
+            const float4 p = a.part[row * a.segs + i];
+            const float3 two[2] = {make_float3(r.m, r.s, r.u), make_float3(p.x, p.y, p.z)};
+            const float3 j = join(two, 2, a.c);
+            r.m = j.x, r.s = j.y, r.u = j.z;
         }
+        // the shares are about their exact maxima: no rounding of m c to take out, which wave_join's correction would add
+        const float M = wave_max(r.m);
+        const float D = (r.m - M) * a.c, f = exp2_hw(D);
+        const bool some = r.s != 0.0f;
+        const float3 p = make_float3(M, wave_sum(some ? r.s * f : 0.0f), wave_sum(some ? __builtin_fmaf(D, r.s, r.u) * f : 0.0f));
+        __syncthreads();
+        if ((threadIdx.x & 63u) == 0) sh.part[threadIdx.x >> 6] = p;
+        __syncthreads();
+        const float3 j = join(sh.part, NT / WAVE, a.c);
+        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, sh, [](uint32_t) { return false; });
+        score_out<E>(a, row, x, st);
         if (a.k) {
-            top_radix(a.C, a.k, sh, [&](uint32_t i) { return top_key(E::get(x[i]), i); });
-            if (threadIdx.x < a.k) {
-                const uint32_t i = top_index(sh.key[threadIdx.x]);
-                a.top_labels[row * a.k + threadIdx.x] = (int32_t)i;
-                a.top_logprobs[row * a.k + threadIdx.x] = logprob(E::get(x[i]));
+            const uint32_t n = a.segs * a.k;
+            const uint64_t *keys = a.part_key + row * n;
+            auto out = [&](uint32_t rank, uint64_t key) {
+                a.top_labels[row * a.k + rank] = (int32_t)top_index(key);
+                a.top_logprobs[row * a.k + rank] = logprob_of<E>(a, st, top_value(key));
+            };
+            bool few = n <= NT;
+            uint32_t got = n;
+            if (few) {
+                __syncthreads();
+                if (threadIdx.x < n) top.key[threadIdx.x] = keys[threadIdx.x];
+            } else {
+                uint32_t mine = 0;
+                for (uint32_t i = threadIdx.x; i < n; i += NT) {
+                    const uint32_t o = (uint32_t)(keys[i] >> 24);
+                    mine = o > mine ? o : mine;
+                }
+                const uint32_t tau = top_threshold<NT>(mine, a.k, sh, top);
+                for (uint32_t i = threadIdx.x; i < n; i += NT)
+                    if ((uint32_t)(keys[i] >> 24) >= tau) push_candidate(keys[i], sh, top);
+                __syncthreads();
+                got = sh.count;
+                few = got >= a.k && got <= TOP_CAP;
             }
+            __syncthreads();
+            if (few) rank_candidates<NT>(got, a.k, top, out);
+            else top_radix<NT>(n, a.k, sh, top, [&](uint32_t i) { return keys[i]; }, out);
             __syncthreads();
         }
     }
 }
 
-// What the gradient of a row looks like: scale * p_i * (a + b * log2 p_i) everywhere (p of the streamed classes), and at the
-// n listed classes id[] the values val[], which are final.
+// ------------------------------------------------------------------------------------------
+// gradients
+// ------------------------------------------------------------------------------------------
+// What the gradient of a row looks like: p_i (a + b log2 p_i), p of the streamed classes, everywhere but at the n listed classes
+// sh.id[], where sh.val[] are the final values.
 struct RowGrad {
     float m, l2, a, b;
     uint32_t n;
-};
-
-struct ScoreGradArgs {
-    const void *logits;
-    size_t rows, stride;
-    uint32_t C, k;
-    float c, inv_t;
-    const int32_t *labels, *top_labels;
-    const float4 *stats;
-    const float *up_logprobs, *up_entropy, *up_top;
-    void *grad;
 };
 
 // A class that is listed twice gets the sum of its entries; only its first entry writes.
@@ -238,36 +636,93 @@ __device__ __forceinline__ bool first_entry(const LogitsLds &sh, uint32_t j, uin
     return true;
 }
 
-template <class E>
-__device__ void write_grad(const RowGrad &g, const typename E::raw *x, typename E::raw *out, uint32_t C, float c, LogitsLds &sh)
+template <class E, int NT>
+__device__ void zero_classes(typename E::raw *out, uint32_t n)
 {
-    const bool none = g.m == -INFINITY;                      // no streamed class has any probability
-    for (uint32_t i = threadIdx.x; i < C; i += LG_THREADS) {
-        const float t = (E::get(x[i]) - g.m) * c - g.l2;
-        out[i] = E::put(none ? 0.0f : exp2_hw(t) * (g.a + g.b * vmax(t, T_FLOOR)));
+    constexpr int VEC = E::VEC;
+    const uint32_t nvec = n / VEC;
+    for (uint32_t i = threadIdx.x; i < nvec; i += NT) store_raw<E>(out + (size_t)i * VEC, u32x4{0, 0, 0, 0});
+    if (threadIdx.x < n - nvec * VEC) out[nvec * VEC + threadIdx.x] = E::put(0.0f);
+}
+
+// The gradient at the n classes x .. of a row, whose indices start at first.
+template <class E, int NT, int U, bool ENT>
+__device__ __forceinline__ void write_grad(const RowGrad &g, const typename E::raw *x, typename E::raw *out, uint32_t n, uint32_t first, float c,
+                                           const LogitsLds &sh)
+{
+    constexpr int VEC = E::VEC;
+    if (g.m == -INFINITY) {                                  // no streamed class has any probability
+        zero_classes<E, NT>(out, n);
+    } else {
+        auto value = [&](float v) {
+            const float t = (v - g.m) * c - g.l2;
+            return exp2_hw(t) * (ENT ? __builtin_fmaf(g.b, vmax(t, T_FLOOR), g.a) : g.a);
+        };
+        const uint32_t nvec = n / VEC;
+        uint32_t i = threadIdx.x;
+        for (; i + (U - 1) * NT < nvec; i += U * NT) {
+            u32x4 w[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) w[k] = load_raw<E>(x + (size_t)(i + k * NT) * VEC);
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                float v[VEC];
+                E::unpack(w[k], v);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
+                store_raw<E>(out + (size_t)(i + k * NT) * VEC, E::pack(v));
+            }
+        }
+        for (; i < nvec; i += NT) {
+            float v[VEC];
+            E::unpack(load_raw<E>(x + (size_t)i * VEC), v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
+            store_raw<E>(out + (size_t)i * VEC, E::pack(v));
+        }
+        if (threadIdx.x < n - nvec * VEC) out[nvec * VEC + threadIdx.x] = E::put(value(E::get(x[nvec * VEC + threadIdx.x])));
     }
     __syncthreads();                                         // the block's own stores before the listed classes' (same addresses)
-    for (uint32_t j = threadIdx.x; j < g.n; j += LG_THREADS)
-        if (sh.id[j] >= 0) out[sh.id[j]] = E::put(sh.val[j]);
+    for (uint32_t j = threadIdx.x; j < g.n; j += NT) {
+        const uint32_t at = (uint32_t)sh.id[j] - first;
+        if (sh.id[j] >= 0 && at < n) out[at] = E::put(sh.val[j]);
+    }
     __syncthreads();
 }
 
-template <class E>
-__global__ __launch_bounds__(LG_THREADS) void score_grad_kernel(ScoreGradArgs a)
+struct ScoreGradArgs {
+    const void *logits;
+    size_t rows, stride;
+    uint32_t C, k;
+    float c, inv_t;
+    const int32_t *labels, *top_labels;
+    const float4 *stats;
+    const float *up_logprobs, *up_entropy, *up_top;
+    void *grad;
+    uint32_t segs, seg;
+};
+
+template <class E, int NT, bool ENT>
+__global__ __launch_bounds__(NT) void score_grad_kernel(ScoreGradArgs a)
 {
     __shared__ LogitsLds sh;
-    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const size_t work = a.rows * a.segs;
+    for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
+        const size_t row = a.segs == 1 ? w : w / a.segs;
+        const uint32_t first = a.segs == 1 ? 0 : (uint32_t)(w - row * a.segs) * a.seg;
+        const uint32_t len = a.C - first < a.seg ? a.C - first : a.seg;
         const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        typename E::raw *out = (typename E::raw *)a.grad + row * a.C;
+        typename E::raw *out = (typename E::raw *)a.grad + row * a.C + first;
         const float4 st = a.stats[row];
         if (st.x == -INFINITY) {                             // an empty row has constant outputs
-            for (uint32_t i = threadIdx.x; i < a.C; i += LG_THREADS) out[i] = E::put(0.0f);
+            zero_classes<E, NT>(out, len);
             continue;
         }
         const uint32_t n = a.k + 1;
-        const float gh = a.up_entropy ? a.up_entropy[row] : 0.0f;
+        const float gh = ENT ? a.up_entropy[row] : 0.0f;
         __syncthreads();
-        for (uint32_t j = threadIdx.x; j < n; j += LG_THREADS) {
+        if (threadIdx.x < n) {
+            const uint32_t j = threadIdx.x;
             int32_t id = -1;
             float v = 0.0f;
             if (j == a.k) {
@@ -278,9 +733,8 @@ __global__ __launch_bounds__(LG_THREADS) void score_grad_kernel(ScoreGradArgs a)
             sh.val[j] = (uint32_t)id < a.C ? v : 0.0f;
         }
         __syncthreads();
-        float part = 0.0f;
-        for (uint32_t j = threadIdx.x; j < n; j += LG_THREADS) part += sh.val[j];
-        const float total = block_sum(part, sh);
+        float total = 0.0f;
+        for (uint32_t j = 0; j < n; ++j) total += sh.val[j];
         // d/dx_i = (1/T) [ sum_j g_j [i = id_j] - p_i (G + gH (log p_i + H)) ]
         RowGrad g = {st.x, st.y, -a.inv_t * (total + gh * st.z), -a.inv_t * gh * LN2, n};
         float val = 0.0f;
@@ -296,10 +750,13 @@ __global__ __launch_bounds__(LG_THREADS) void score_grad_kernel(ScoreGradArgs a)
         __syncthreads();
         if (threadIdx.x < n) sh.id[threadIdx.x] = id, sh.val[threadIdx.x] = val;
         __syncthreads();
-        write_grad<E>(g, x, out, a.C, a.c, sh);
+        write_grad<E, NT, 16 / E::VEC, ENT>(g, x + first, out, len, first, a.c, sh);
     }
 }
 
+// ------------------------------------------------------------------------------------------
+// distillation
+// ------------------------------------------------------------------------------------------
 struct DistillArgs {
     const void *logits;
     size_t rows, stride;
@@ -314,9 +771,11 @@ struct DistillArgs {
     const float *up;
     int up_rows;
     void *grad;
+    uint32_t segs, seg;
+    float4 *part;                                // [rows, segs] shares of a split row
 };
 
-// The list's terms of one row, thread j < K holding entry j (K <= LG_THREADS).  Renormalised: q = softmax of the teacher's values
+// The list's terms of one row, thread j < K holding entry j (K <= NT).  Renormalised: q = softmax of the teacher's values
 // over the listed classes and st describes all of the student's classes.  Bucket: q = exp(teacher), the teacher's remaining mass
 // q0 = 1 - sum q against the student's mass p0 off the list, and st describes the classes OFF the list; all classes follow by
 // adding the listed ones, so neither p0 nor the rest's gradient suffers the cancellation of 1 - sum p.
@@ -328,8 +787,8 @@ struct ListTerms {
     bool rest;           // the bucket takes part
 };
 
-template <class E>
-__device__ ListTerms list_terms(const DistillArgs &a, size_t row, const typename E::raw *x, const RowStats &st, LogitsLds &sh)
+template <class E, int NT>
+__device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, size_t row, const typename E::raw *x, const RowStats &st, LogitsLds &sh)
 {
     // sh.id / sh.val: the valid ids and their q on return
     const uint32_t j = threadIdx.x;
@@ -343,19 +802,20 @@ __device__ ListTerms list_terms(const DistillArgs &a, size_t row, const typename
     float q = 0.0f, logq = 0.0f;
     ListTerms r = {0.0f, st.m, st.l2, 0.0f, 0.0f, 0.0f, false};
     if (!a.bucket) {
-        const float tm = block_max(t, sh);
+        const float tm = block_max<NT>(t, sh);
         if (tm > -INFINITY) {
             const float e = id >= 0 ? exp2_hw((t - tm) * LOG2E) : 0.0f;
-            const float tt = block_sum(e, sh);
+            const float tt = block_sum<NT>(e, sh);
             q = e / tt;
             logq = (t - tm) - LN2 * log2_hw(tt);
             r.mass = 1.0f;
         }
     } else {
+        // 1 - sum q in double: where the teacher's list holds nearly everything, little is left of it
         const double qd = id >= 0 ? exp((double)t) : 0.0;
         q = (float)qd;
         logq = t;
-        const double sum = block_sum_f64(qd, sh);
+        const double sum = block_sum_f64<NT>(qd, sh);
         const double q0 = 1.0 - sum > 0.0 ? 1.0 - sum : 0.0;
         r.rest = st.m > -INFINITY;
         r.q0 = (float)q0;
@@ -367,11 +827,11 @@ __device__ ListTerms list_terms(const DistillArgs &a, size_t row, const typename
     if (a.bucket) {
         float dummy;
         const bool counts = j < a.K && id >= 0 && first_entry(sh, j, a.K, dummy);
-        const float top = block_max(counts ? v : -INFINITY, sh);
+        const float top = block_max<NT>(counts ? v : -INFINITY, sh);
         const float M = vmax(st.m, top);
         if (M > -INFINITY) {
             const float rest = r.rest ? exp2_hw((st.m - M) * a.c + st.l2) : 0.0f;
-            const float s = block_sum(counts ? exp2_hw((v - M) * a.c) : 0.0f, sh) + rest;
+            const float s = block_sum<NT>(counts ? exp2_hw((v - M) * a.c) : 0.0f, sh) + rest;
             r.m = M;
             r.l2 = log2_hw(s);
             r.p0 = rest / s;
@@ -384,29 +844,50 @@ __device__ ListTerms list_terms(const DistillArgs &a, size_t row, const typename
         if (st.m != st.m) r.m = st.m;
     }
     const float logp = (v - r.m) * a.inv_t - LN2 * r.l2;
-    r.loss += block_sum(q > 0.0f || q != q ? q * (logq - logp) : 0.0f, sh);
+    r.loss += block_sum<NT>(q > 0.0f || q != q ? q * (logq - logp) : 0.0f, sh);
     return r;
 }
 
-template <class E>
-__device__ RowStats distill_stats(const DistillArgs &a, size_t row, const typename E::raw *x, LogitsLds &sh)
+// Marks the listed classes among the n from `first` on: bit e of mask[v] for element e of vector v.
+template <class E, int NT>
+__device__ __forceinline__ void mask_listed(const DistillArgs &a, size_t row, uint32_t first, uint32_t n, uint32_t *mask)
 {
-    if (!a.bucket) return row_stats<E>(x, a.C, a.c, sh, [](uint32_t) { return false; });
+    constexpr int VEC = E::VEC;
+    const uint32_t words = (n / VEC + 1 + 3) / 4;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < words; i += NT) mask[i] = 0;
+    __syncthreads();
+    if (threadIdx.x < a.K) {
+        const uint32_t at = (uint32_t)a.ids[row * a.K + threadIdx.x] - first;
+        if (at < n) {
+            const uint32_t v = at / VEC, e = at % VEC;
+            atomicOr(&mask[v >> 2], 1u << ((v & 3u) * 8 + e));
+        }
+    }
+    __syncthreads();
+}
+
+// Where one pass did not do: statistics of a row's classes, the listed ones left out for the bucket.
+template <class E, int NT>
+__device__ RowStats distill_careful(const DistillArgs &a, size_t row, const typename E::raw *x, LogitsLds &sh)
+{
+    if (!a.bucket) return careful_stats<E, NT>(x, a.C, a.c, sh, [](uint32_t) { return false; });
     __syncthreads();
     if (threadIdx.x < a.K) sh.id[threadIdx.x] = a.ids[row * a.K + threadIdx.x];
     __syncthreads();
-    return row_stats<E>(x, a.C, a.c, sh, [&](uint32_t i) {
+    return careful_stats<E, NT>(x, a.C, a.c, sh, [&](uint32_t i) {
         for (uint32_t j = 0; j < a.K; ++j)
             if (sh.id[j] == (int32_t)i) return true;
         return false;
     });
 }
 
-template <class E>
-__device__ void distill_grad(const DistillArgs &a, size_t row, const typename E::raw *x, const RowStats &st, const ListTerms &r,
-                             float up, LogitsLds &sh)
+// The gradient at n classes from `first` on, out being theirs.
+template <class E, int NT>
+__device__ __forceinline__ void distill_grad(const DistillArgs &a, size_t row, const typename E::raw *x, uint32_t first, uint32_t n,
+                                             const RowStats &st, const ListTerms &r, float up, LogitsLds &sh)
 {
-    typename E::raw *out = (typename E::raw *)a.grad + row * a.C;
+    typename E::raw *out = (typename E::raw *)a.grad + row * a.C + first;
     const float coef = (a.weights ? a.weights[row] : 1.0f) * a.t * a.scale * up;
     const uint32_t j = threadIdx.x;
     int32_t id = -1;
@@ -422,40 +903,100 @@ __device__ void distill_grad(const DistillArgs &a, size_t row, const typename E:
     if (j < a.K) sh.id[j] = id, sh.val[j] = val;
     __syncthreads();
     const float dense = a.bucket ? r.p0 * r.mass - r.q0 : r.mass;
-    write_grad<E>(RowGrad{st.m, st.l2, coef * dense, 0.0f, a.K}, x, out, a.C, a.c, sh);
+    write_grad<E, NT, 16 / E::VEC, false>(RowGrad{st.m, st.l2, coef * dense, 0.0f, a.K}, x + first, out, n, first, a.c, sh);
 }
 
-// MODE 0: losses (and statistics), 1: losses and gradient, 2: gradient from the forward call's statistics
-template <class E, int MODE>
-__global__ __launch_bounds__(LG_THREADS) void distill_rows_kernel(DistillArgs a)
+// Loss (and gradient) of a row once its statistics are there.
+template <class E, int NT, bool LOSS, bool GRAD>
+__device__ __forceinline__ void distill_row(const DistillArgs &a, size_t row, const typename E::raw *x, uint32_t first, uint32_t n, bool ignored,
+                                            const RowStats &st, LogitsLds &sh)
 {
+    ListTerms r = {};
+    bool dead = ignored;
+    if (!dead) {
+        r = list_terms<E, NT>(a, row, x, st, sh);
+        dead = r.m == -INFINITY;                             // no class has any probability
+    }
+    if (LOSS && threadIdx.x == 0) {
+        a.out_rows[row] = dead ? 0.0f : (a.weights ? a.weights[row] : 1.0f) * a.t * a.t * r.loss;
+        if (a.stats) a.stats[row] = make_float4(st.m, st.l2, 0.0f, 0.0f);
+    }
+    if (GRAD) {
+        if (dead) zero_classes<E, NT>((typename E::raw *)a.grad + row * a.C + first, n);
+        else distill_grad<E, NT>(a, row, x, first, n, st, r, LOSS || !a.up ? 1.0f : a.up[a.up_rows ? row : 0], sh);
+    }
+}
+
+constexpr uint32_t MASK_VECS = 32768;            // vectors of a bucket segment: 32 KB of mask
+
+// One block per row or per segment of a row; GRAD (whole rows): the row is read again for its gradient.
+template <class E, int NT, bool BUCKET, bool GRAD>
+__global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a)
+{
+    constexpr int U = 32 / E::VEC;
+    __shared__ LogitsLds sh;
+    extern __shared__ uint32_t mask[];
+    const size_t work = a.rows * a.segs;
+    for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
+        const size_t row = a.segs == 1 ? w : w / a.segs;
+        const uint32_t first = a.segs == 1 ? 0 : (uint32_t)(w - row * a.segs) * a.seg;
+        const uint32_t n = a.C - first < a.seg ? a.C - first : a.seg;
+        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
+        const bool ignored = a.weights && a.weights[row] == 0.0f;    // 0 whatever it holds
+        RowStats st = {-INFINITY, -INFINITY, 0.0f};
+        if (!ignored) {
+            if (BUCKET) mask_listed<E, NT>(a, row, first, n, mask);
+            const Running r = scan_classes<E, NT, U, false, BUCKET>(x + first, n, a.c, (const uint8_t *)mask);
+            const float3 j = block_join<NT>(r, a.c, sh);
+            if (a.segs > 1) {
+                if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, 0.0f, 0.0f);
+                continue;
+            }
+            st = row_ok(j) ? stats_of(j) : distill_careful<E, NT>(a, row, x, sh);
+        } else if (a.segs > 1)
+            continue;
+        distill_row<E, NT, true, GRAD>(a, row, x, 0, a.C, ignored, st, sh);
+        __syncthreads();
+    }
+}
+
+template <class E>
+__global__ __launch_bounds__(JOIN_THREADS) void distill_join_kernel(DistillArgs a)
+{
+    constexpr int NT = JOIN_THREADS;
     __shared__ LogitsLds sh;
     for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        const float w = a.weights ? a.weights[row] : 1.0f;
-        bool dead = w == 0.0f;                               // an ignored row: 0 whatever it holds
+        const bool ignored = a.weights && a.weights[row] == 0.0f;
         RowStats st = {-INFINITY, -INFINITY, 0.0f};
-        ListTerms r = {};
-        if (!dead) {
-            if (MODE == 2) {
-                const float4 f = a.stats[row];
-                st = {f.x, f.y, 0.0f};
-            } else
-                st = distill_stats<E>(a, row, x, sh);
-            r = list_terms<E>(a, row, x, st, sh);
-            dead = r.m == -INFINITY;                         // no class has any probability
+        if (!ignored) {
+            float3 j = make_float3(M_START, 0.0f, 0.0f);
+            for (uint32_t i = 0; i < a.segs; ++i) {
+                const float4 p = a.part[row * a.segs + i];
+                const float3 two[2] = {j, make_float3(p.x, p.y, 0.0f)};
+                j = join(two, 2, a.c);
+            }
+            st = row_ok(j) ? stats_of(j) : distill_careful<E, NT>(a, row, x, sh);
         }
-        if (MODE != 2 && threadIdx.x == 0) {
-            a.out_rows[row] = dead ? 0.0f : w * a.t * a.t * r.loss;
-            if (a.stats) a.stats[row] = make_float4(st.m, st.l2, 0.0f, 0.0f);
-        }
-        if (MODE != 0) {
-            if (dead) {
-                typename E::raw *out = (typename E::raw *)a.grad + row * a.C;
-                for (uint32_t i = threadIdx.x; i < a.C; i += LG_THREADS) out[i] = E::put(0.0f);
-            } else
-                distill_grad<E>(a, row, x, st, r, MODE == 2 ? a.up[a.up_rows ? row : 0] : 1.0f, sh);
-        }
+        distill_row<E, NT, true, false>(a, row, x, 0, a.C, ignored, st, sh);
+        __syncthreads();
+    }
+}
+
+// The gradient from the statistics of an earlier launch, one block per row or per segment of a row.
+template <class E, int NT>
+__global__ __launch_bounds__(NT) void distill_grad_kernel(DistillArgs a)
+{
+    __shared__ LogitsLds sh;
+    const size_t work = a.rows * a.segs;
+    for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
+        const size_t row = a.segs == 1 ? w : w / a.segs;
+        const uint32_t first = a.segs == 1 ? 0 : (uint32_t)(w - row * a.segs) * a.seg;
+        const uint32_t n = a.C - first < a.seg ? a.C - first : a.seg;
+        const float4 f = a.stats[row];
+        const RowStats st = {f.x, f.y, 0.0f};
+        distill_row<E, NT, false, true>(a, row, (const typename E::raw *)a.logits + row * a.stride, first, n,
+                                        a.weights && a.weights[row] == 0.0f, st, sh);
         __syncthreads();
     }
 }
@@ -496,7 +1037,30 @@ static int logits_check(const char *name, const void *logits, int dtype, size_t 
     return 0;
 }
 
-static dim3 row_grid(size_t rows) { return dim3((uint32_t)(rows < 1u << 20 ? rows : 1u << 20)); }
+static dim3 work_grid(size_t work) { return dim3((uint32_t)(work < 1u << 20 ? work : 1u << 20)); }
+
+// How a row's classes are dealt out to blocks: whole rows where there are enough of them to fill the chip, else segments of at
+// least 4096 classes so that about `blocks` blocks run.  A segment is a multiple of 8 classes and holds at most `most`.
+struct Split {
+    uint32_t segs, seg;
+};
+static Split split_rows(size_t rows, uint32_t C, uint32_t blocks, uint32_t most)
+{
+    if (rows == 0) return {1, C};
+    uint32_t segs = rows >= blocks ? 1 : (uint32_t)((blocks + rows - 1) / rows);
+    const uint32_t fit = C / 4096 ? C / 4096 : 1, need = (C + most - 1) / most;
+    segs = segs < fit ? segs : fit;
+    segs = segs > need ? segs : need;
+    uint32_t seg = segs == 1 ? C : (((C + segs - 1) / segs + 7) & ~7u);
+    if (seg > most && segs > 1) seg = most;
+    return {(C + seg - 1) / seg, seg};
+}
+constexpr uint32_t FILL_BLOCKS = 1024;
+static Split score_split(size_t rows, uint32_t C) { return split_rows(rows, C, FILL_BLOCKS, 1u << 24); }
+static Split distill_split(size_t rows, uint32_t C, int dtype)
+{
+    return split_rows(rows, C, FILL_BLOCKS, (MASK_VECS - 8) * (dtype == ODBOX_DTYPE_F32 ? 4 : 8));
+}
 
 #define LOGITS_LAUNCH(dtype, K_, ...)                                                       \
     do {                                                                                    \
@@ -513,8 +1077,9 @@ extern "C" {
 
 size_t odbox_label_logprobs_workspace(size_t rows, int C, int top_k)
 {
-    (void)rows, (void)C, (void)top_k;
-    return 0;
+    if (C < 1 || top_k < 0) return 0;
+    const Split sp = score_split(rows, (uint32_t)C);
+    return sp.segs == 1 ? 0 : rows * sp.segs * (sizeof(float4) + (size_t)top_k * sizeof(uint64_t));
 }
 
 int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size_t row_stride, const int32_t *labels, int top_k,
@@ -529,10 +1094,18 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
     if (top_k && (!out_top_logprobs || !out_top_labels)) return fail(ODBOX_EINVAL, "%s: top_k = %d, NULL top output", name, top_k);
     if (!aligned16(out_stats)) return fail(ODBOX_EINVAL, "%s: out_stats must be 16-byte aligned", name);
     if (workspace_bytes < odbox_label_logprobs_workspace(rows, C, top_k)) return fail(ODBOX_ENOSPC, "%s: workspace too small", name);
-    (void)workspace;
-    ScoreArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)top_k, LOG2E / temperature, 1.0f / temperature, labels, out_logprobs, out_entropy,
-                   out_top_logprobs, out_top_labels, (float4 *)out_stats};
-    LOGITS_LAUNCH(dtype, score_rows_kernel<E>, row_grid(rows), dim3(LG_THREADS), 0, (hipStream_t)stream, a);
+    if (!aligned16(workspace)) return fail(ODBOX_EINVAL, "%s: workspace must be 16-byte aligned", name);
+    const Split sp = score_split(rows, (uint32_t)C);
+    if (sp.segs > 1 && !workspace) return fail(ODBOX_EINVAL, "%s: NULL workspace", name);
+    float4 *part = (float4 *)workspace;
+    ScoreArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)top_k, LOG2E / temperature, 1.0f / temperature, labels, out_logprobs,
+                   out_entropy, out_top_logprobs, out_top_labels, (float4 *)out_stats, sp.segs, sp.seg, part,
+                   (uint64_t *)(part + (sp.segs > 1 ? rows * sp.segs : 0))};
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 grid = work_grid(rows * sp.segs);
+    if (top_k) LOGITS_LAUNCH(dtype, (score_kernel<E, 256, true>), grid, dim3(256), 0, st, a);
+    else LOGITS_LAUNCH(dtype, (score_kernel<E, 256, false>), grid, dim3(256), 0, st, a);
+    if (sp.segs > 1) LOGITS_LAUNCH(dtype, score_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);
     return launch_status("label_logprobs");
 }
 
@@ -549,9 +1122,12 @@ int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, in
     if ((uintptr_t)grad % (dtype == ODBOX_DTYPE_F32 ? 4 : 2)) return fail(ODBOX_EINVAL, "%s: grad is not aligned to its element", name);
     if (upstream_logprobs && !labels) return fail(ODBOX_EINVAL, "%s: upstream_logprobs without labels", name);
     if (upstream_top && top_k && !top_labels) return fail(ODBOX_EINVAL, "%s: upstream_top without top_labels", name);
+    const Split sp = score_split(rows, (uint32_t)C);
     ScoreGradArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)(upstream_top ? top_k : 0), LOG2E / temperature, 1.0f / temperature,
-                       labels, top_labels, (const float4 *)stats, upstream_logprobs, upstream_entropy, upstream_top, grad};
-    LOGITS_LAUNCH(dtype, score_grad_kernel<E>, row_grid(rows), dim3(LG_THREADS), 0, (hipStream_t)stream, a);
+                       labels, top_labels, (const float4 *)stats, upstream_logprobs, upstream_entropy, upstream_top, grad, sp.segs, sp.seg};
+    const dim3 grid = work_grid(rows * sp.segs);
+    if (upstream_entropy) LOGITS_LAUNCH(dtype, (score_grad_kernel<E, 256, true>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    else LOGITS_LAUNCH(dtype, (score_grad_kernel<E, 256, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
     return launch_status("label_logprobs_backward");
 }
 
@@ -568,8 +1144,11 @@ static int distill_check(const char *name, const void *logits, int dtype, size_t
 
 size_t odbox_distill_loss_workspace(size_t rows, int C, int K)
 {
-    (void)C, (void)K;
-    return rows * sizeof(float) + SUM_BLOCKS * sizeof(double) + 16;
+    (void)K;
+    if (C < 1) return 0;
+    // blocks of the sum, row losses, row statistics and shares of split rows (the smaller segments of float32)
+    const Split sp = distill_split(rows, (uint32_t)C, ODBOX_DTYPE_F32);
+    return SUM_BLOCKS * sizeof(double) + ((rows + 3) / 4) * 4 * sizeof(float) + (sp.segs > 1 ? rows * (sp.segs + 1) * sizeof(float4) : 0);
 }
 
 int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t row_stride, const float *teacher_logprobs,
@@ -593,10 +1172,27 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
     if (!workspace) return fail(ODBOX_EINVAL, "%s: NULL workspace", name);
     double *partial = (double *)workspace;
     float *per_row = out_rows ? out_rows : (float *)(partial + SUM_BLOCKS);
-    DistillArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)K, LOG2E / temperature, temperature, 1.0f / temperature, scale, rest, teacher_logprobs,
-                     teacher_labels, row_weights, per_row, (float4 *)out_stats, nullptr, 0, grad};
-    if (grad) LOGITS_LAUNCH(dtype, (distill_rows_kernel<E, 1>), row_grid(rows), dim3(LG_THREADS), 0, st, a);
-    else LOGITS_LAUNCH(dtype, (distill_rows_kernel<E, 0>), row_grid(rows), dim3(LG_THREADS), 0, st, a);
+    const Split sp = distill_split(rows, (uint32_t)C, dtype);
+    float4 *spare = (float4 *)((float *)(partial + SUM_BLOCKS) + (rows + 3) / 4 * 4);
+    float4 *keep = out_stats ? (float4 *)out_stats : sp.segs > 1 ? spare : nullptr;
+    DistillArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)K, LOG2E / temperature, temperature, 1.0f / temperature, scale, rest,
+                     teacher_logprobs, teacher_labels, row_weights, per_row, keep, nullptr, 0, grad, sp.segs, sp.seg, spare + rows};
+    const dim3 grid = work_grid(rows * sp.segs);
+    const size_t lds = rest == ODBOX_REST_BUCKET ? (sp.seg / (dtype == ODBOX_DTYPE_F32 ? 4 : 8) + 8) & ~3u : 0;
+    const bool fused = grad && sp.segs == 1;
+    if (rest == ODBOX_REST_BUCKET) {
+        if (fused) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true, true>), grid, dim3(256), lds, st, a);
+        else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true, false>), grid, dim3(256), lds, st, a);
+    } else {
+        if (fused) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false, true>), grid, dim3(256), lds, st, a);
+        else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false, false>), grid, dim3(256), lds, st, a);
+    }
+    if (sp.segs > 1) {
+        LOGITS_LAUNCH(dtype, distill_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);
+        if (grad) {
+            LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, 256>), grid, dim3(256), 0, st, a);
+        }
+    }
     if (int rc = launch_status("distill_loss")) return rc;
     if (out_loss) {
         const size_t run = sum_run(rows), nb = (rows + run - 1) / run;
@@ -620,9 +1216,10 @@ int odbox_distill_loss_backward(const void *logits, int dtype, size_t rows, int 
     if (rows == 0) return 0;
     if (!stats || !upstream || !grad) return fail(ODBOX_EINVAL, "%s: NULL stats, upstream or grad", name);
     if (!aligned16(stats)) return fail(ODBOX_EINVAL, "%s: stats must be 16-byte aligned", name);
+    const Split sp = distill_split(rows, (uint32_t)C, dtype);
     DistillArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)K, LOG2E / temperature, temperature, 1.0f / temperature, scale, rest, teacher_logprobs,
-                     teacher_labels, row_weights, nullptr, (float4 *)stats, upstream, upstream_rows, grad};
-    LOGITS_LAUNCH(dtype, (distill_rows_kernel<E, 2>), row_grid(rows), dim3(LG_THREADS), 0, (hipStream_t)stream, a);
+                     teacher_labels, row_weights, nullptr, (float4 *)stats, upstream, upstream_rows, grad, sp.segs, sp.seg, nullptr};
+    LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, 256>), work_grid(rows * sp.segs), dim3(256), 0, (hipStream_t)stream, a);
     return launch_status("distill_loss_backward");
 }
 

@@ -52,6 +52,16 @@ def test_bad_arguments_are_refused(lib):
     assert lib.odbox_distill_loss_backward(*dict(dist_b, rows=0, logits=None).values()) == 0
 
 
+def test_workspace_queries(lib):
+    for rows in (0, 1, 7, 4096, 1 << 40):
+        for C in (1, 80, 4097, 131072, 1 << 24):
+            assert lib.odbox_label_logprobs_workspace(rows, C, 1) >= lib.odbox_label_logprobs_workspace(rows, C, 0) >= 0
+            assert lib.odbox_distill_loss_workspace(rows, C, 128) >= 4 * rows
+    for C in (0, -5):
+        assert lib.odbox_label_logprobs_workspace(4, C, 1) == 0 and lib.odbox_distill_loss_workspace(4, C, 1) == 0
+    assert lib.odbox_label_logprobs_workspace(4, 100, -1) == 0
+
+
 def test_signatures():
     def params(f):
         return list(inspect.signature(f).parameters)
