@@ -31,6 +31,7 @@ struct Unaligned {
 };
 struct F32 {
     using raw = float;
+    static __device__ __forceinline__ u32x4 none() { return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}; }   // -inf
     static constexpr int VEC = 4;
     static __device__ __forceinline__ float get(raw v) { return v; }
     static __device__ __forceinline__ raw put(float v) { return v; }
@@ -46,6 +47,7 @@ struct F32 {
 };
 struct F16 {
     using raw = _Float16;
+    static __device__ __forceinline__ u32x4 none() { return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u}; }
     static constexpr int VEC = 8;
     static __device__ __forceinline__ float get(raw v) { return (float)v; }
     static __device__ __forceinline__ raw put(float v) { return (_Float16)v; }
@@ -65,6 +67,7 @@ struct F16 {
 };
 struct BF16 {
     using raw = uint16_t;
+    static __device__ __forceinline__ u32x4 none() { return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
     static constexpr int VEC = 8;
     static __device__ __forceinline__ float get(raw v) { return __uint_as_float((uint32_t)v << 16); }
     static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(raw, (__bf16)v); }
@@ -135,17 +138,17 @@ constexpr uint32_t LIST_MAX = ODBOX_MAX_TOP + 1;
 
 // What one block shares.
 struct LogitsLds {
-    double d[MAX_WAVES];
     float f[MAX_WAVES];
     float3 part[MAX_WAVES];
     uint32_t count;
     uint32_t pick[2];
-    int32_t id[LIST_MAX];
-    float val[LIST_MAX];
+    alignas(16) int32_t id[LIST_MAX + 3];        // listed classes; -1: none, or listed before
+    float val[LIST_MAX], x[LIST_MAX];
+    float sum[4];
 };
 struct TopLds {
-    uint32_t group[256];                         // group maxima of the selection; the radix histogram
-    uint64_t key[TOP_CAP];
+    alignas(16) uint32_t group[256];             // group maxima of the selection; the radix histogram
+    uint64_t key[TOP_CAP];                       // candidates; while they are collected, TOP_CAP / waves to each wave
 };
 
 template <int NT, class Op>
@@ -164,20 +167,6 @@ template <int NT>
 __device__ __forceinline__ float block_max(float v, LogitsLds &sh) { return block_reduce<NT>(v, -INFINITY, sh, [](float a, float b) { return vmax(a, b); }); }
 template <int NT>
 __device__ __forceinline__ float block_sum(float v, LogitsLds &sh) { return block_reduce<NT>(v, 0.0f, sh, [](float a, float b) { return a + b; }); }
-template <int NT>
-__device__ __forceinline__ double block_sum_f64(double v, LogitsLds &sh)
-{
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) sh.d[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh.d[0];
-#pragma unroll
-    for (int w = 1; w < NT / WAVE; ++w) v += sh.d[w];
-    return v;
-}
-
 // ------------------------------------------------------------------------------------------
 // softmax statistics of a row
 // ------------------------------------------------------------------------------------------
@@ -256,10 +245,16 @@ __device__ __forceinline__ RowStats stats_of(const float3 &j)
     return {j.x, l2, LN2 * (l2 - j.z / j.y)};
 }
 
-// Two passes over the row by the whole block, for the rows that are not row_ok.  skip(i): class i is left out.
-template <class E, int NT, class Skip>
-__device__ __attribute__((noinline)) RowStats careful_stats(const typename E::raw *x, uint32_t C, float c, LogitsLds &sh, Skip skip)
+// Two passes over the row by the whole block, for the rows that are not row_ok; the classes among the K of sh.id are left out.
+// (A call, so that it costs the kernels no registers.)
+template <class E, int NT>
+__device__ __attribute__((noinline)) RowStats careful_stats(const typename E::raw *x, uint32_t C, float c, uint32_t K, LogitsLds &sh)
 {
+    auto skip = [&](uint32_t i) {
+        for (uint32_t j = 0; j < K; ++j)
+            if (sh.id[j] == (int32_t)i) return true;
+        return false;
+    };
     float m = -INFINITY, bad = 0.0f;
     for (uint32_t i = threadIdx.x; i < C; i += NT) {
         const float v = E::get(x[i]);
@@ -347,22 +342,32 @@ __device__ __forceinline__ float top_value(uint64_t k)
 }
 
 // n candidates in top.key, unordered, the k largest of the whole among them: each counts the larger ones, out(rank, key) is
-// called for the first k.
+// called for the first k.  Where there are more threads than candidates, 2^sh lanes share one.
 template <int NT, class Out>
 __device__ __forceinline__ void rank_candidates(uint32_t n, uint32_t k, const TopLds &top, Out out)
 {
-    for (uint32_t t = threadIdx.x; t < n; t += NT) {
-        const uint64_t mine = top.key[t];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += top.key[j] > mine;
-        if (rank < k) out(rank, mine);
+    uint32_t sh = 0;
+    while (sh < 6 && (n << (sh + 1)) <= NT) ++sh;
+    const uint32_t lanes = 1u << sh, sub = threadIdx.x & (lanes - 1), step = NT >> sh;
+    for (uint32_t t0 = 0; t0 < n; t0 += step) {
+        const uint32_t t = t0 + (threadIdx.x >> sh);
+        const uint64_t mine = top.key[t < n ? t : 0];
+        uint32_t rank = 0, j = sub;
+        for (; j + 3 * lanes < n; j += 4 * lanes) {
+            const uint64_t p = top.key[j], q = top.key[j + lanes], r = top.key[j + 2 * lanes], w = top.key[j + 3 * lanes];
+            rank += (p > mine) + (q > mine) + (r > mine) + (w > mine);
+        }
+        for (; j < n; j += lanes) rank += top.key[j] > mine;
+        for (uint32_t off = 1; off < lanes; off <<= 1) rank += __shfl_xor(rank, off);
+        if (t < n && sub == 0 && rank < k) out(rank, mine);
     }
 }
 
 // The k (<= ODBOX_MAX_TOP, <= n) largest of n unique keys: the k-th key by a radix selection of eight bits a pass, then exactly k
 // keys are collected.  Right for every input, eight passes: where the threshold below keeps too few or too many candidates.
-template <int NT, class Key, class Out>
-__device__ __attribute__((noinline)) void top_radix(uint32_t n, uint32_t k, LogitsLds &sh, TopLds &top, Key key, Out out)
+// They end up in top.key in order.  (A call: key is a plain object.)
+template <int NT, class Key>
+__device__ __attribute__((noinline)) void top_radix(uint32_t n, uint32_t k, LogitsLds &sh, TopLds &top, Key key)
 {
     uint64_t prefix = 0;
     uint32_t want = k;
@@ -393,34 +398,46 @@ __device__ __attribute__((noinline)) void top_radix(uint32_t n, uint32_t k, Logi
         if (q >= prefix) top.key[atomicAdd(&sh.count, 1u)] = q;       // unique keys: exactly k of them
     }
     __syncthreads();
-    rank_candidates<NT>(k, k, top, out);
+    uint64_t mine[(ODBOX_MAX_TOP + NT - 1) / NT];
+    uint32_t rank[(ODBOX_MAX_TOP + NT - 1) / NT];
+#pragma unroll
+    for (uint32_t h = 0; h < (ODBOX_MAX_TOP + NT - 1) / NT; ++h) {
+        const uint32_t t = threadIdx.x + h * NT;
+        mine[h] = t < k ? top.key[t] : 0;
+        rank[h] = 0;
+        for (uint32_t j = 0; j < k; ++j) rank[h] += top.key[j] > mine[h];
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t h = 0; h < (ODBOX_MAX_TOP + NT - 1) / NT; ++h)
+        if (threadIdx.x + h * NT < k) top.key[rank[h]] = mine[h];
     __syncthreads();
 }
+template <class E>
+struct ClassKey {
+    const typename E::raw *x;
+    uint32_t first;
+    __device__ __forceinline__ uint64_t operator()(uint32_t i) const { return top_key(E::get(x[i]), first + i); }
+};
+struct StoredKey {
+    const uint64_t *keys;
+    __device__ __forceinline__ uint64_t operator()(uint32_t i) const { return keys[i]; }
+};
 
-// A value (in f32_ordered form) that at least k of the row's classes reach and few more do: the k-th largest of 64 or 256 group
-// maxima, a group being the classes of NT / 64 or NT / 256 neighbouring threads (>= 2 k groups keep about 1.4 k candidates of
-// values in no particular order).  mine: the thread's largest value.
+// Groups of the threshold: at least 2 k of them keep about 1.4 k candidates of values in no particular order.
+__device__ __forceinline__ uint32_t top_groups(uint32_t k) { return k <= 32 ? 64 : k <= 64 ? 128 : 256; }
+
+// A value (in f32_ordered form) that at least k of the row's classes reach and few more do: the k-th largest of G group maxima,
+// which the caller has put into top.group.
 template <int NT>
-__device__ __forceinline__ uint32_t top_threshold(uint32_t mine, uint32_t k, LogitsLds &sh, TopLds &top)
+__device__ __forceinline__ uint32_t top_threshold(uint32_t G, uint32_t k, LogitsLds &sh, TopLds &top)
 {
-    auto fold = [&](int lanes) {
-        uint32_t v = mine;
-        for (int off = 1; off < lanes; off <<= 1) {
-            const uint32_t o = __shfl_xor(v, off);
-            v = o > v ? o : v;
-        }
-        return v;
-    };
-    const uint32_t G = k <= 32 ? 64 : 256;
-    const uint32_t lanes = NT / G;
-    const uint32_t v = fold((int)lanes);
-    __syncthreads();
-    if (threadIdx.x % lanes == 0) top.group[threadIdx.x / lanes] = v;
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    if (threadIdx.x < G) {
-        const uint32_t w = top.group[threadIdx.x];
+    for (uint32_t t = threadIdx.x; t < G; t += NT) {
+        const uint32_t w = top.group[t];
         uint32_t gt = 0, ge = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < G; j += 4) {
             const uint4 q = *(const uint4 *)&top.group[j];
             gt += (q.x > w) + (q.y > w) + (q.z > w) + (q.w > w);
@@ -437,53 +454,141 @@ __device__ __forceinline__ void push_candidate(uint64_t key, LogitsLds &sh, TopL
     if (at < TOP_CAP) top.key[at] = key;
 }
 
-// The k best of the n classes at x, whose indices start at first.  m: the thread's largest value in scan_classes' order of work, so
-// only threads that hold a candidate look at their classes again.
-template <class E, int NT, int U, class Out>
-__device__ __forceinline__ void top_classes(const typename E::raw *x, uint32_t n, uint32_t first, uint32_t k, float m, bool ok, LogitsLds &sh,
-                                            TopLds &top, Out out)
+// A row, or a segment of one, in the registers of NT threads: vector i of the n / VEC whole ones at thread i % NT, one of the
+// remaining classes at each of the first threads.  What is read twice (the top classes, a gradient) is read from memory once.
+template <class E, int NT>
+struct Resident {
+    static constexpr int R = 16, VEC = E::VEC, N = 16, STEP = N / VEC;       // N values at a time
+    using raw = typename E::raw;
+    u32x4 w[R];
+    float tail;
+    uint32_t tid;
+    static constexpr uint32_t CAP = (uint32_t)R * NT * VEC;
+
+    __device__ __forceinline__ void load(const raw *x, uint32_t n)
+    {
+        const uint32_t nvec = n / VEC;
+        forget_thread();
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const uint32_t i = k * NT + tid;
+            w[k] = E::none();
+            if (i < nvec) w[k] = load_raw<E>(x + (size_t)i * VEC);
+        }
+        tail = threadIdx.x < n - nvec * VEC ? E::get(x[nvec * VEC + threadIdx.x]) : -INFINITY;
+    }
+    // The thread's number as something new: what is computed from it (an index for every value) is not kept from row to row.
+    __device__ __forceinline__ void forget_thread()
+    {
+        tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+    }
+    // Keeps the compiler from holding the unpacked values (two to one register) between two uses of the row.
+    __device__ __forceinline__ void forget()
+    {
+        forget_thread();
+#pragma unroll
+        for (int k = 0; k < R; ++k) asm volatile("" : "+v"(w[k]));
+    }
+    // f(k, v): N values from vector k on, for the steps that hold any
+    template <class F>
+    __device__ __forceinline__ void each(uint32_t n, F f) const
+    {
+        const uint32_t nvec = n / VEC;
+#pragma unroll
+        for (int k = 0; k < R; k += STEP) {
+            if ((uint32_t)k * NT < nvec) {
+                float v[N];
+#pragma unroll
+                for (int j = 0; j < STEP; ++j) E::unpack(w[k + j], v + j * VEC);
+                f(k, v);
+            }
+        }
+    }
+};
+
+// The k best of the n classes in r, whose indices start at first; m: the thread's largest value.
+template <class E, int NT, class Out>
+__device__ __forceinline__ void top_classes(const Resident<E, NT> &r, const typename E::raw *x, uint32_t n, uint32_t first, uint32_t k, float m,
+                                            bool ok, LogitsLds &sh, TopLds &top, Out out)
 {
-    constexpr int VEC = E::VEC;
+    using Row = Resident<E, NT>;
+    constexpr int VEC = E::VEC, WAVES = NT / WAVE;
+    constexpr uint32_t ROOM = TOP_CAP / WAVES;
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
     bool few = false;
     if (ok) {
-        const uint32_t tau = top_threshold<NT>(f32_ordered(m), k, sh, top);
-        const float floor_ = f32_unordered(tau);
-        if (m >= floor_) {
-            const uint32_t nvec = n / VEC;
-            uint32_t i = threadIdx.x;
-            auto look = [&](float v, uint32_t at) {
-                if (v >= floor_) push_candidate(top_key(v, first + at), sh, top);
-            };
-            for (; i + (U - 1) * NT < nvec; i += U * NT) {
-                u32x4 w[U];
-#pragma unroll
-                for (int j = 0; j < U; ++j) w[j] = load_raw<E>(x + (size_t)(i + j * NT) * VEC);
-#pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    float v[VEC], g = -INFINITY;
-                    E::unpack(w[j], v);
-#pragma unroll
-                    for (int e = 0; e < VEC; e += 2) g = vmax3(g, v[e], v[e + 1]);
-                    if (g >= floor_)
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) look(v[e], (i + j * NT) * VEC + e);
-                }
-            }
-            for (; i < nvec; i += NT) {
-                float v[VEC];
-                E::unpack(load_raw<E>(x + (size_t)i * VEC), v);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) look(v[e], i * VEC + e);
-            }
-            if (threadIdx.x < n - nvec * VEC) look(E::get(x[nvec * VEC + threadIdx.x]), nvec * VEC + threadIdx.x);
-        }
+        // group maxima: of neighbouring threads, or of parts of a thread's values where there are too few threads
+        const uint32_t G = top_groups(k);
         __syncthreads();
-        const uint32_t got = sh.count;
-        few = got >= k && got <= TOP_CAP;
-        if (few) rank_candidates<NT>(got, k, top, out);
+        if (NT >= 256 || G == 64) {
+            const uint32_t lanes = NT / G;
+            uint32_t v = f32_ordered(m);
+            for (uint32_t off = 1; off < lanes; off <<= 1) {
+                const uint32_t o = __shfl_xor(v, off);
+                v = o > v ? o : v;
+            }
+            if (threadIdx.x % lanes == 0) top.group[threadIdx.x / lanes] = v;
+        } else {
+            // a single wave and k > 32: the values of a thread fall into four groups, or into two
+            float g[4] = {r.tail, M_START, M_START, M_START};
+            r.each(n, [&](int kk, const float *v) {
+#pragma unroll
+                for (int j = 0; j < Resident<E, NT>::N; ++j) g[(kk + j / VEC) & 3] = vmax(g[(kk + j / VEC) & 3], v[j]);
+            });
+            if (G == 128) g[0] = vmax(g[0], g[2]), g[1] = vmax(g[1], g[3]);
+            for (uint32_t part = 0; part < G / 64; ++part)
+                top.group[part * 64 + threadIdx.x] = f32_ordered(vmax(part == 0 ? g[0] : part == 1 ? g[1] : part == 2 ? g[2] : g[3], M_START));
+        }
+        const float tau = f32_unordered(top_threshold<NT>(G, k, sh, top));
+        // candidates by wave: a ballot per value, so positions need no atomics and their order no luck
+        uint32_t have = 0;
+        auto look = [&](float v, uint32_t at) {
+            const uint64_t hit = __ballot(v >= tau);
+            if (hit == 0) return;
+            const uint32_t pos = have + __builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0u));
+            if (v >= tau && pos < ROOM) top.key[wave * ROOM + pos] = top_key(v, first + at);
+            have += __popcll(hit);
+        };
+        if (__any(m >= tau)) {
+            r.each(n, [&](int kk, const float *v) {
+#pragma unroll
+                for (int j = 0; j < Resident<E, NT>::N; ++j) look(v[j], ((kk + j / VEC) * NT + r.tid) * VEC + j % VEC);
+            });
+            look(r.tail, n / VEC * VEC + threadIdx.x);
+        }
+        // the waves' lists side by side (places beyond the row's end hold -inf, tau is M_START or more: they never count)
+        const bool over = have > ROOM;
+        if (WAVES > 1) {
+            uint64_t mine[(ROOM + 63) / 64];
+#pragma unroll
+            for (uint32_t i = 0; i < (ROOM + 63) / 64; ++i)
+                if (i * 64 + lane < have && !over) mine[i] = top.key[wave * ROOM + i * 64 + lane];
+            if (lane == 0) sh.f[wave] = over ? 1e9f : (float)have;
+            __syncthreads();
+            uint32_t base = 0, all = 0;
+            for (int i = 0; i < WAVES; ++i) {
+                const uint32_t c = sh.f[i] > 1e8f ? 2 * TOP_CAP : (uint32_t)sh.f[i];
+                if ((uint32_t)i < wave) base += c;
+                all += c;
+            }
+            few = all >= k && all <= TOP_CAP;
+            if (few)
+#pragma unroll
+                for (uint32_t i = 0; i < (ROOM + 63) / 64; ++i)
+                    if (i * 64 + lane < have) top.key[base + i * 64 + lane] = mine[i];
+            have = all;
+        } else
+            few = have >= k && !over;
+        __syncthreads();
+        if (few) rank_candidates<NT>(have, k, top, out);
         __syncthreads();
     }
-    if (!few) top_radix<NT>(n, k, sh, top, [&](uint32_t i) { return top_key(E::get(x[i]), first + i); }, out);
+    if (!few) {
+        top_radix<NT>(n, k, sh, top, ClassKey<E>{x, first});
+        for (uint32_t t = threadIdx.x; t < k; t += NT) out(t, top.key[t]);
+        __syncthreads();
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -520,36 +625,67 @@ __device__ __forceinline__ void score_out(const ScoreArgs &a, size_t row, const 
     if (a.stats) a.stats[row] = make_float4(st.m, st.l2, st.ent, 0.0f);
 }
 
-// One block per row or per segment of a row.
-template <class E, int NT, bool TOP>
+// A piece of work: a row, or one of its segments.
+struct Piece {
+    size_t row;
+    uint32_t first, n;
+};
+__device__ __forceinline__ Piece piece_of(size_t w, uint32_t segs, uint32_t seg, uint32_t C)
+{
+    const size_t row = segs == 1 ? w : w / segs;
+    const uint32_t first = segs == 1 ? 0 : (uint32_t)(w - row * segs) * seg;
+    return {row, first, C - first < seg ? C - first : seg};
+}
+
+// Without top classes: the row streams by.
+template <class E, int NT>
 __global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a)
 {
-    constexpr int U = 32 / E::VEC;               // 64 (float32: 128) bytes of loads in flight per thread
+    __shared__ LogitsLds sh;
+    const size_t work = a.rows * a.segs;
+    for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
+        const Piece p = piece_of(w, a.segs, a.seg, a.C);
+        const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
+        const Running r = scan_classes<E, NT, 32 / E::VEC, true, false>(x + p.first, p.n, a.c, nullptr);
+        const float3 j = block_join<NT>(r, a.c, sh);
+        if (a.segs > 1) {
+            if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, j.z, 0.0f);
+            continue;
+        }
+        score_out<E>(a, p.row, x, row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, 0, sh));
+    }
+}
+
+// With top classes: the row stays in registers.
+template <class E, int NT>
+__global__ __launch_bounds__(NT, 4) void score_top_kernel(ScoreArgs a)
+{
     __shared__ LogitsLds sh;
     __shared__ TopLds top;
     const size_t work = a.rows * a.segs;
     for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
-        const size_t row = a.segs == 1 ? w : w / a.segs;
-        const uint32_t seg = a.segs == 1 ? 0 : (uint32_t)(w - row * a.segs), first = seg * a.seg;
-        const uint32_t n = a.C - first < a.seg ? a.C - first : a.seg;
-        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        const Running r = scan_classes<E, NT, U, true, false>(x + first, n, a.c, nullptr);
+        const Piece p = piece_of(w, a.segs, a.seg, a.C);
+        const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
+        Resident<E, NT> reg;
+        reg.load(x + p.first, p.n);
+        Running r = running_start(a.c);
+        reg.each(p.n, [&](int, const float *v) { absorb<Resident<E, NT>::N, true>(v, a.c, r); });
+        absorb<1, true>(&reg.tail, a.c, r);
+        reg.forget();
         const float3 j = block_join<NT>(r, a.c, sh);
         const bool ok = row_ok(j);
         if (a.segs > 1) {
             if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, j.z, 0.0f);
-            if (TOP) {
-                const uint32_t k = a.k < n ? a.k : n;        // a short last segment fills up with keys below every class's
-                for (uint32_t t = k + threadIdx.x; t < a.k; t += NT) a.part_key[w * a.k + t] = 0;
-                top_classes<E, NT, U>(x + first, n, first, k, r.m, ok, sh, top, [&](uint32_t rank, uint64_t key) { a.part_key[w * a.k + rank] = key; });
-            }
+            const uint32_t k = a.k < p.n ? a.k : p.n;        // a short last segment fills up with keys below every class's
+            for (uint32_t t = k + threadIdx.x; t < a.k; t += NT) a.part_key[w * a.k + t] = 0;
+            top_classes<E, NT>(reg, x + p.first, p.n, p.first, k, r.m, ok, sh, top, [&](uint32_t rank, uint64_t key) { a.part_key[w * a.k + rank] = key; });
             continue;
         }
-        const RowStats st = ok ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, sh, [](uint32_t) { return false; });
-        score_out<E>(a, row, x, st);
-        if (TOP) top_classes<E, NT, U>(x, n, 0, a.k, r.m, ok, sh, top, [&](uint32_t rank, uint64_t key) {
-            a.top_labels[row * a.k + rank] = (int32_t)top_index(key);
-            a.top_logprobs[row * a.k + rank] = logprob_of<E>(a, st, top_value(key));
+        const RowStats st = ok ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, 0, sh);
+        score_out<E>(a, p.row, x, st);
+        top_classes<E, NT>(reg, x, p.n, 0, a.k, r.m, ok, sh, top, [&](uint32_t rank, uint64_t key) {
+            a.top_labels[p.row * a.k + rank] = (int32_t)top_index(key);
+            a.top_logprobs[p.row * a.k + rank] = logprob_of<E>(a, st, top_value(key));
         });
     }
 }
@@ -580,7 +716,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void score_join_kernel(ScoreArgs a)
         if ((threadIdx.x & 63u) == 0) sh.part[threadIdx.x >> 6] = p;
         __syncthreads();
         const float3 j = join(sh.part, NT / WAVE, a.c);
-        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, sh, [](uint32_t) { return false; });
+        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, 0, sh);
         score_out<E>(a, row, x, st);
         if (a.k) {
             const uint32_t n = a.segs * a.k;
@@ -600,7 +736,14 @@ __global__ __launch_bounds__(JOIN_THREADS) void score_join_kernel(ScoreArgs a)
                     const uint32_t o = (uint32_t)(keys[i] >> 24);
                     mine = o > mine ? o : mine;
                 }
-                const uint32_t tau = top_threshold<NT>(mine, a.k, sh, top);
+                const uint32_t G = top_groups(a.k), lanes = NT / G;
+                for (uint32_t off = 1; off < lanes; off <<= 1) {
+                    const uint32_t o = __shfl_xor(mine, off);
+                    mine = o > mine ? o : mine;
+                }
+                __syncthreads();
+                if (threadIdx.x % lanes == 0) top.group[threadIdx.x / lanes] = mine;
+                const uint32_t tau = top_threshold<NT>(G, a.k, sh, top);
                 for (uint32_t i = threadIdx.x; i < n; i += NT)
                     if ((uint32_t)(keys[i] >> 24) >= tau) push_candidate(keys[i], sh, top);
                 __syncthreads();
@@ -609,7 +752,10 @@ __global__ __launch_bounds__(JOIN_THREADS) void score_join_kernel(ScoreArgs a)
             }
             __syncthreads();
             if (few) rank_candidates<NT>(got, a.k, top, out);
-            else top_radix<NT>(n, a.k, sh, top, [&](uint32_t i) { return keys[i]; }, out);
+            else {
+                top_radix<NT>(n, a.k, sh, top, StoredKey{keys});
+                for (uint32_t t = threadIdx.x; t < a.k; t += NT) out(t, top.key[t]);
+            }
             __syncthreads();
         }
     }
@@ -618,13 +764,6 @@ __global__ __launch_bounds__(JOIN_THREADS) void score_join_kernel(ScoreArgs a)
 // ------------------------------------------------------------------------------------------
 // gradients
 // ------------------------------------------------------------------------------------------
-// What the gradient of a row looks like: p_i (a + b log2 p_i), p of the streamed classes, everywhere but at the n listed classes
-// sh.id[], where sh.val[] are the final values.
-struct RowGrad {
-    float m, l2, a, b;
-    uint32_t n;
-};
-
 // A class that is listed twice gets the sum of its entries; only its first entry writes.
 __device__ __forceinline__ bool first_entry(const LogitsLds &sh, uint32_t j, uint32_t n, float &sum)
 {
@@ -647,49 +786,42 @@ __device__ void zero_classes(typename E::raw *out, uint32_t n)
     if (threadIdx.x < n - nvec * VEC) out[nvec * VEC + threadIdx.x] = E::put(0.0f);
 }
 
-// The gradient at the n classes x .. of a row, whose indices start at first.
+// out = p (ga + gb log2 p) at n classes of a row, p by the row's statistics.
 template <class E, int NT, int U, bool ENT>
-__device__ __forceinline__ void write_grad(const RowGrad &g, const typename E::raw *x, typename E::raw *out, uint32_t n, uint32_t first, float c,
-                                           const LogitsLds &sh)
+__device__ __forceinline__ void write_grad(const RowStats &st, float ga, float gb, const typename E::raw *x, typename E::raw *out, uint32_t n, float c)
 {
     constexpr int VEC = E::VEC;
-    if (g.m == -INFINITY) {                                  // no streamed class has any probability
+    if (st.m == -INFINITY) {                                 // no class has any probability
         zero_classes<E, NT>(out, n);
-    } else {
-        auto value = [&](float v) {
-            const float t = (v - g.m) * c - g.l2;
-            return exp2_hw(t) * (ENT ? __builtin_fmaf(g.b, vmax(t, T_FLOOR), g.a) : g.a);
-        };
-        const uint32_t nvec = n / VEC;
-        uint32_t i = threadIdx.x;
-        for (; i + (U - 1) * NT < nvec; i += U * NT) {
-            u32x4 w[U];
+        return;
+    }
+    auto value = [&](float v) {
+        const float t = (v - st.m) * c - st.l2;
+        return exp2_hw(t) * (ENT ? __builtin_fmaf(gb, vmax(t, T_FLOOR), ga) : ga);
+    };
+    const uint32_t nvec = n / VEC;
+    uint32_t i = threadIdx.x;
+    for (; i + (U - 1) * NT < nvec; i += U * NT) {
+        u32x4 w[U];
 #pragma unroll
-            for (int k = 0; k < U; ++k) w[k] = load_raw<E>(x + (size_t)(i + k * NT) * VEC);
+        for (int k = 0; k < U; ++k) w[k] = load_raw<E>(x + (size_t)(i + k * NT) * VEC);
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                float v[VEC];
-                E::unpack(w[k], v);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
-                store_raw<E>(out + (size_t)(i + k * NT) * VEC, E::pack(v));
-            }
-        }
-        for (; i < nvec; i += NT) {
+        for (int k = 0; k < U; ++k) {
             float v[VEC];
-            E::unpack(load_raw<E>(x + (size_t)i * VEC), v);
+            E::unpack(w[k], v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
-            store_raw<E>(out + (size_t)i * VEC, E::pack(v));
+            store_raw<E>(out + (size_t)(i + k * NT) * VEC, E::pack(v));
         }
-        if (threadIdx.x < n - nvec * VEC) out[nvec * VEC + threadIdx.x] = E::put(value(E::get(x[nvec * VEC + threadIdx.x])));
     }
-    __syncthreads();                                         // the block's own stores before the listed classes' (same addresses)
-    for (uint32_t j = threadIdx.x; j < g.n; j += NT) {
-        const uint32_t at = (uint32_t)sh.id[j] - first;
-        if (sh.id[j] >= 0 && at < n) out[at] = E::put(sh.val[j]);
+    for (; i < nvec; i += NT) {
+        float v[VEC];
+        E::unpack(load_raw<E>(x + (size_t)i * VEC), v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
+        store_raw<E>(out + (size_t)i * VEC, E::pack(v));
     }
-    __syncthreads();
+    if (threadIdx.x < n - nvec * VEC) out[nvec * VEC + threadIdx.x] = E::put(value(E::get(x[nvec * VEC + threadIdx.x])));
 }
 
 struct ScoreGradArgs {
@@ -710,27 +842,25 @@ __global__ __launch_bounds__(NT) void score_grad_kernel(ScoreGradArgs a)
     __shared__ LogitsLds sh;
     const size_t work = a.rows * a.segs;
     for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
-        const size_t row = a.segs == 1 ? w : w / a.segs;
-        const uint32_t first = a.segs == 1 ? 0 : (uint32_t)(w - row * a.segs) * a.seg;
-        const uint32_t len = a.C - first < a.seg ? a.C - first : a.seg;
-        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        typename E::raw *out = (typename E::raw *)a.grad + row * a.C + first;
-        const float4 st = a.stats[row];
-        if (st.x == -INFINITY) {                             // an empty row has constant outputs
-            zero_classes<E, NT>(out, len);
+        const Piece p = piece_of(w, a.segs, a.seg, a.C);
+        const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
+        typename E::raw *out = (typename E::raw *)a.grad + p.row * a.C + p.first;
+        const float4 f = a.stats[p.row];
+        const RowStats st = {f.x, f.y, f.z};
+        if (st.m == -INFINITY) {                             // an empty row has constant outputs
+            zero_classes<E, NT>(out, p.n);
             continue;
         }
         const uint32_t n = a.k + 1;
-        const float gh = ENT ? a.up_entropy[row] : 0.0f;
+        const float gh = ENT ? a.up_entropy[p.row] : 0.0f;
         __syncthreads();
-        if (threadIdx.x < n) {
-            const uint32_t j = threadIdx.x;
+        for (uint32_t j = threadIdx.x; j < n; j += NT) {
             int32_t id = -1;
             float v = 0.0f;
             if (j == a.k) {
-                if (a.up_logprobs && (uint32_t)a.labels[row] < a.C) id = a.labels[row], v = a.up_logprobs[row];
-            } else if (a.up_top)
-                id = a.top_labels[row * a.k + j], v = a.up_top[row * a.k + j];
+                if (a.up_logprobs) id = a.labels[p.row], v = a.up_logprobs[p.row];
+            } else
+                id = a.top_labels[p.row * a.k + j], v = a.up_top[p.row * a.k + j];
             sh.id[j] = (uint32_t)id < a.C ? id : -1;
             sh.val[j] = (uint32_t)id < a.C ? v : 0.0f;
         }
@@ -738,21 +868,16 @@ __global__ __launch_bounds__(NT) void score_grad_kernel(ScoreGradArgs a)
         float total = 0.0f;
         for (uint32_t j = 0; j < n; ++j) total += sh.val[j];
         // d/dx_i = (1/T) [ sum_j g_j [i = id_j] - p_i (G + gH (log p_i + H)) ]
-        RowGrad g = {st.x, st.y, -a.inv_t * (total + gh * st.z), -a.inv_t * gh * LN2, n};
-        float val = 0.0f;
-        int32_t id = -1;
-        if (threadIdx.x < n && sh.id[threadIdx.x] >= 0) {
+        const float ga = -a.inv_t * (total + gh * st.ent), gb = -a.inv_t * gh * LN2;
+        write_grad<E, NT, 16 / E::VEC, ENT>(st, ga, gb, x + p.first, out, p.n, a.c);
+        __syncthreads();                                     // the block's own stores before the listed classes' (same addresses)
+        for (uint32_t j = threadIdx.x; j < n; j += NT) {
+            const uint32_t at = (uint32_t)sh.id[j] - p.first;
             float sum;
-            if (first_entry(sh, threadIdx.x, n, sum)) {
-                id = sh.id[threadIdx.x];
-                const float t = (E::get(x[id]) - st.x) * a.c - st.y;
-                val = a.inv_t * sum + exp2_hw(t) * (g.a + g.b * vmax(t, T_FLOOR));
-            }
+            if (sh.id[j] < 0 || at >= p.n || !first_entry(sh, j, n, sum)) continue;
+            const float t = (E::get(x[sh.id[j]]) - st.m) * a.c - st.l2;
+            out[at] = E::put(a.inv_t * sum + exp2_hw(t) * __builtin_fmaf(gb, vmax(t, T_FLOOR), ga));
         }
-        __syncthreads();
-        if (threadIdx.x < n) sh.id[threadIdx.x] = id, sh.val[threadIdx.x] = val;
-        __syncthreads();
-        write_grad<E, NT, 16 / E::VEC, ENT>(g, x + first, out, len, first, a.c, sh);
     }
 }
 
@@ -777,76 +902,139 @@ struct DistillArgs {
     float4 *part;                                // [rows, segs] shares of a split row
 };
 
-// The list's terms of one row, thread j < K holding entry j (K <= NT).  Renormalised: q = softmax of the teacher's values
-// over the listed classes and st describes all of the student's classes.  Bucket: q = exp(teacher), the teacher's remaining mass
-// q0 = 1 - sum q against the student's mass p0 off the list, and st describes the classes OFF the list; all classes follow by
-// adding the listed ones, so neither p0 nor the rest's gradient suffers the cancellation of 1 - sum p.
-struct ListTerms {
-    float loss;          // of the row, before weight and T^2
-    float m, l2;         // all classes
-    float mass;          // sum q (+ q0)
-    float p0, q0;
-    bool rest;           // the bucket takes part
+// The list of one row.  Renormalised: q = softmax of the teacher's values over the listed classes, and the statistics describe all of
+// the student's classes.  Bucket: q = exp(teacher), the teacher's remaining mass q0 = 1 - sum q against the student's mass p0
+// off the list, and the statistics describe the classes OFF the list; all classes follow by adding the listed ones, so neither
+// p0 nor the rest's gradient suffers the cancellation of 1 - sum p.
+//
+// Everything that needs no statistics is done by the block's first wave while the row is on its way: entries lane and lane + 64.
+struct ListEntry {
+    float q, logq, x;
+    bool on;
 };
 
-template <class E, int NT>
-__device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, size_t row, const typename E::raw *x, const RowStats &st, LogitsLds &sh)
+// exp(t) to about 2^-23 relative for t <= 0: the product with log2(e) in two parts
+__device__ __forceinline__ float exp_split(float t)
 {
-    // sh.id / sh.val: the valid ids and their q on return
-    const uint32_t j = threadIdx.x;
-    int32_t id = -1;
-    float t = -INFINITY, v = -INFINITY;
-    if (j < a.K) {
-        id = a.ids[row * a.K + j];
-        if ((uint32_t)id >= a.C) id = -1;
-        if (id >= 0) t = a.teacher[row * a.K + j], v = E::get(x[id]);
-    }
-    float q = 0.0f, logq = 0.0f;
-    ListTerms r = {0.0f, st.m, st.l2, 0.0f, 0.0f, 0.0f, false};
-    if (!a.bucket) {
-        const float tm = block_max<NT>(t, sh);
-        if (tm > -INFINITY) {
-            const float e = id >= 0 ? exp2_hw((t - tm) * LOG2E) : 0.0f;
-            const float tt = block_sum<NT>(e, sh);
-            q = e / tt;
-            logq = (t - tm) - LN2 * log2_hw(tt);
-            r.mass = 1.0f;
+    const float hi = t * LOG2E;
+    if (!(hi > -150.0f)) return t != t ? t : 0.0f;
+    const float lo = __builtin_fmaf(t, LOG2E, -hi) + t * 1.925963033500e-08f;      // LOG2E is log2(e) less that
+    return exp2_hw(hi) * __builtin_fmaf(lo, LN2, 1.0f);
+}
+
+// Fills sh.id (first entries of their classes; -1 otherwise), sh.val (a class's q, summed over its entries), sh.x (the student's
+// logits there) and sh.sum: sum q, q0, and for the bucket the listed classes' maximum and sum about it.
+template <class E>
+__device__ __forceinline__ void prepare_list(const DistillArgs &a, size_t row, const typename E::raw *x, LogitsLds &sh, ListEntry (&en)[2])
+{
+    const uint32_t lane = threadIdx.x;
+    int32_t id[2];
+    float t[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t j = lane + 64 * h;
+        id[h] = -1;
+        t[h] = -INFINITY;
+        en[h] = {0.0f, -INFINITY, -INFINITY, false};
+        if (j < a.K) {
+            id[h] = a.ids[row * a.K + j];
+            t[h] = a.teacher[row * a.K + j];
         }
+        if ((uint32_t)id[h] < a.C) en[h].on = true, en[h].x = E::get(x[id[h]]);
+        else id[h] = -1, t[h] = -INFINITY;
+        sh.id[j] = id[h];
+    }
+    if (lane < 3) sh.id[128 + lane] = -1;
+    float mass, q0 = 0.0f;
+    if (!a.bucket) {
+        const float tm = wave_max(vmax(t[0], t[1]));
+        float e[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) e[h] = en[h].on && tm > -INFINITY ? exp2_hw((t[h] - tm) * LOG2E) : 0.0f;
+        const float tt = wave_sum(e[0] + e[1]), logt = LN2 * log2_hw(tt);
+        mass = tm > -INFINITY ? 1.0f : 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (tm > -INFINITY) en[h].q = e[h] / tt, en[h].logq = (t[h] - tm) - logt;
     } else {
-        // 1 - sum q in double: where the teacher's list holds nearly everything, little is left of it
-        const double qd = id >= 0 ? exp((double)t) : 0.0;
-        q = (float)qd;
-        logq = t;
-        const double sum = block_sum_f64<NT>(qd, sh);
-        const double q0 = 1.0 - sum > 0.0 ? 1.0 - sum : 0.0;
-        r.rest = st.m > -INFINITY;
-        r.q0 = (float)q0;
-        r.mass = (float)(r.rest ? sum + q0 : sum);
+        double sum = 0.0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            en[h].q = en[h].on ? exp_split(t[h]) : 0.0f;
+            en[h].logq = t[h];
+            sum += (double)en[h].q;
+        }
+        for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+        const double left = 1.0 - sum;           // in double: where the list holds nearly everything, little is left of it
+        q0 = left > 0.0 ? (float)left : left != left ? NAN : 0.0f;
+        mass = (float)sum;
     }
-    __syncthreads();
-    if (j < a.K) sh.id[j] = id, sh.val[j] = q;
-    __syncthreads();
-    if (a.bucket) {
-        float dummy;
-        const bool counts = j < a.K && id >= 0 && first_entry(sh, j, a.K, dummy);
-        const float top = block_max<NT>(counts ? v : -INFINITY, sh);
-        const float M = vmax(st.m, top);
-        if (M > -INFINITY) {
-            const float rest = r.rest ? exp2_hw((st.m - M) * a.c + st.l2) : 0.0f;
-            const float s = block_sum<NT>(counts ? exp2_hw((v - M) * a.c) : 0.0f, sh) + rest;
-            r.m = M;
-            r.l2 = log2_hw(s);
-            r.p0 = rest / s;
-            if (r.rest && r.q0 > 0.0f) {
-                const float logp0 = (st.m - M) * a.inv_t + LN2 * (st.l2 - r.l2);
-                r.loss = r.q0 * (LN2 * log2_hw(r.q0) - logp0);
+    // entries of a class listed before
+    bool first[2] = {en[0].on, en[1].on};
+    bool twice = false;
+    for (uint32_t i = 0; i < a.K; i += 4) {
+        const int4 o = *(const int4 *)&sh.id[i];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t j = lane + 64 * h;
+            if ((o.x == id[h] && i < j) || (o.y == id[h] && i + 1 < j) || (o.z == id[h] && i + 2 < j) || (o.w == id[h] && i + 3 < j)) {
+                twice |= first[h];
+                first[h] = false;
             }
-        } else
-            r.m = M;
-        if (st.m != st.m) r.m = st.m;
+        }
     }
-    const float logp = (v - r.m) * a.inv_t - LN2 * r.l2;
-    r.loss += block_sum<NT>(q > 0.0f || q != q ? q * (logq - logp) : 0.0f, sh);
+    float q[2] = {en[0].q, en[1].q};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) sh.val[lane + 64 * h] = q[h], sh.x[lane + 64 * h] = en[h].x;
+    if (__any(twice)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (!first[h]) continue;
+            q[h] = 0.0f;
+            for (uint32_t i = 0; i < a.K; ++i)
+                if (sh.id[i] == id[h]) q[h] += sh.val[i];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sh.val[lane + 64 * h] = q[h];
+            if (!first[h]) sh.id[lane + 64 * h] = -1;
+        }
+    }
+    float top = -INFINITY, s = 0.0f;
+    if (a.bucket) {
+        top = wave_max(vmax(first[0] ? en[0].x : -INFINITY, first[1] ? en[1].x : -INFINITY));
+        if (top > -INFINITY)
+            s = wave_sum((first[0] ? exp2_hw((en[0].x - top) * a.c) : 0.0f) + (first[1] ? exp2_hw((en[1].x - top) * a.c) : 0.0f));
+    }
+    if (lane == 0) sh.sum[0] = mass, sh.sum[1] = q0, sh.sum[2] = top, sh.sum[3] = s;
+}
+
+// What follows once the streamed classes' statistics are there; the same in every thread.
+struct ListTerms {
+    float m, l2;         // all classes; m = -inf: none has any probability
+    float mass;          // sum q (+ q0)
+    float dense;         // the gradient off the list, over coefficient and softmax of the streamed classes
+    float rest;          // the bucket's part of the loss
+};
+__device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, const RowStats &st, const LogitsLds &sh)
+{
+    const float mass = sh.sum[0], q0 = sh.sum[1], top = sh.sum[2], s_on = sh.sum[3];
+    ListTerms r = {st.m, st.l2, mass, mass, 0.0f};
+    if (!a.bucket) return r;
+    const bool rest = st.m > -INFINITY;          // the bucket takes part
+    if (rest) r.mass = mass + q0;
+    r.m = vmax(st.m, top);
+    r.l2 = -INFINITY;
+    if (r.m > -INFINITY) {
+        const float off = rest ? exp2_hw((st.m - r.m) * a.c + st.l2) : 0.0f;
+        const float s = (top > -INFINITY ? s_on * exp2_hw((top - r.m) * a.c) : 0.0f) + off;
+        r.l2 = log2_hw(s);
+        r.dense = off / s * r.mass - q0;
+        if (rest && q0 > 0.0f) r.rest = q0 * (LN2 * log2_hw(q0) - (st.m - r.m) * a.inv_t - LN2 * (st.l2 - r.l2));
+        if (q0 != q0) r.rest = q0;
+    }
+    if (st.m != st.m || s_on != s_on) r.m = NAN;
     return r;
 }
 
@@ -859,8 +1047,8 @@ __device__ __forceinline__ void mask_listed(const DistillArgs &a, size_t row, ui
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < words; i += NT) mask[i] = 0;
     __syncthreads();
-    if (threadIdx.x < a.K) {
-        const uint32_t at = (uint32_t)a.ids[row * a.K + threadIdx.x] - first;
+    for (uint32_t j = threadIdx.x; j < a.K; j += NT) {
+        const uint32_t at = (uint32_t)a.ids[row * a.K + j] - first;
         if (at < n) {
             const uint32_t v = at / VEC, e = at % VEC;
             atomicOr(&mask[v >> 2], 1u << ((v & 3u) * 8 + e));
@@ -869,119 +1057,171 @@ __device__ __forceinline__ void mask_listed(const DistillArgs &a, size_t row, ui
     __syncthreads();
 }
 
-// Where one pass did not do: statistics of a row's classes, the listed ones left out for the bucket.
-template <class E, int NT>
-__device__ RowStats distill_careful(const DistillArgs &a, size_t row, const typename E::raw *x, LogitsLds &sh)
+// Loss of a row by the block's first wave.
+__device__ __forceinline__ void loss_out(const DistillArgs &a, size_t row, float w, const RowStats &st, const ListTerms &r, const ListEntry (&en)[2])
 {
-    if (!a.bucket) return careful_stats<E, NT>(x, a.C, a.c, sh, [](uint32_t) { return false; });
-    __syncthreads();
-    if (threadIdx.x < a.K) sh.id[threadIdx.x] = a.ids[row * a.K + threadIdx.x];
-    __syncthreads();
-    return careful_stats<E, NT>(x, a.C, a.c, sh, [&](uint32_t i) {
-        for (uint32_t j = 0; j < a.K; ++j)
-            if (sh.id[j] == (int32_t)i) return true;
-        return false;
-    });
-}
-
-// The gradient at n classes from `first` on, out being theirs.
-template <class E, int NT>
-__device__ __forceinline__ void distill_grad(const DistillArgs &a, size_t row, const typename E::raw *x, uint32_t first, uint32_t n,
-                                             const RowStats &st, const ListTerms &r, float up, LogitsLds &sh)
-{
-    typename E::raw *out = (typename E::raw *)a.grad + row * a.C + first;
-    const float coef = (a.weights ? a.weights[row] : 1.0f) * a.t * a.scale * up;
-    const uint32_t j = threadIdx.x;
-    int32_t id = -1;
-    float val = 0.0f;
-    if (j < a.K && sh.id[j] >= 0) {
-        float sum;
-        if (first_entry(sh, j, a.K, sum)) {
-            id = sh.id[j];
-            val = coef * (exp2_hw((E::get(x[id]) - r.m) * a.c - r.l2) * r.mass - sum);
-        }
-    }
-    __syncthreads();
-    if (j < a.K) sh.id[j] = id, sh.val[j] = val;
-    __syncthreads();
-    const float dense = a.bucket ? r.p0 * r.mass - r.q0 : r.mass;
-    write_grad<E, NT, 16 / E::VEC, false>(RowGrad{st.m, st.l2, coef * dense, 0.0f, a.K}, x + first, out, n, first, a.c, sh);
-}
-
-// Loss (and gradient) of a row once its statistics are there.
-template <class E, int NT, bool LOSS, bool GRAD>
-__device__ __forceinline__ void distill_row(const DistillArgs &a, size_t row, const typename E::raw *x, uint32_t first, uint32_t n, bool ignored,
-                                            const RowStats &st, LogitsLds &sh)
-{
-    ListTerms r = {};
-    bool dead = ignored;
-    if (!dead) {
-        r = list_terms<E, NT>(a, row, x, st, sh);
-        dead = r.m == -INFINITY;                             // no class has any probability
-    }
-    if (LOSS && threadIdx.x == 0) {
-        a.out_rows[row] = dead ? 0.0f : (a.weights ? a.weights[row] : 1.0f) * a.t * a.t * r.loss;
+    float terms = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (en[h].q > 0.0f || en[h].q != en[h].q) terms += en[h].q * (en[h].logq - ((en[h].x - r.m) * a.inv_t - LN2 * r.l2));
+    terms = wave_sum(terms) + r.rest;
+    if (threadIdx.x == 0) {
+        a.out_rows[row] = r.m == -INFINITY ? 0.0f : w * a.t * a.t * terms;
         if (a.stats) a.stats[row] = make_float4(st.m, st.l2, 0.0f, 0.0f);
     }
-    if (GRAD) {
-        if (dead) zero_classes<E, NT>((typename E::raw *)a.grad + row * a.C + first, n);
-        else distill_grad<E, NT>(a, row, x, first, n, st, r, LOSS || !a.up ? 1.0f : a.up[a.up_rows ? row : 0], sh);
+}
+__device__ __forceinline__ void ignored_out(const DistillArgs &a, size_t row)
+{
+    if (threadIdx.x != 0) return;
+    a.out_rows[row] = 0.0f;
+    if (a.stats) a.stats[row] = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+}
+// The final values at the listed classes among the n from `first` on, over what the block has stored there.
+template <class E, int NT>
+__device__ __forceinline__ void listed_grad(const DistillArgs &a, float coef, const ListTerms &r, typename E::raw *out, uint32_t n, uint32_t first,
+                                            const LogitsLds &sh)
+{
+    __syncthreads();                                         // the block's own stores first (same addresses)
+    for (uint32_t j = threadIdx.x; j < a.K; j += NT) {
+        const uint32_t at = (uint32_t)sh.id[j] - first;
+        if (sh.id[j] >= 0 && at < n) out[at] = E::put(coef * (exp2_hw((sh.x[j] - r.m) * a.c - r.l2) * r.mass - sh.val[j]));
     }
+    __syncthreads();
 }
 
 constexpr uint32_t MASK_VECS = 32768;            // vectors of a bucket segment: 32 KB of mask
 
-// One block per row or per segment of a row; GRAD (whole rows): the row is read again for its gradient.
-template <class E, int NT, bool BUCKET, bool GRAD>
+// Losses, one block per row or per segment of a row: the row streams by.
+template <class E, int NT, bool BUCKET>
 __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a)
 {
-    constexpr int U = 32 / E::VEC;
     __shared__ LogitsLds sh;
     extern __shared__ uint32_t mask[];
     const size_t work = a.rows * a.segs;
     for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
-        const size_t row = a.segs == 1 ? w : w / a.segs;
-        const uint32_t first = a.segs == 1 ? 0 : (uint32_t)(w - row * a.segs) * a.seg;
-        const uint32_t n = a.C - first < a.seg ? a.C - first : a.seg;
-        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        const bool ignored = a.weights && a.weights[row] == 0.0f;    // 0 whatever it holds
-        RowStats st = {-INFINITY, -INFINITY, 0.0f};
-        if (!ignored) {
-            if (BUCKET) mask_listed<E, NT>(a, row, first, n, mask);
-            const Running r = scan_classes<E, NT, U, false, BUCKET>(x + first, n, a.c, (const uint8_t *)mask);
-            const float3 j = block_join<NT>(r, a.c, sh);
-            if (a.segs > 1) {
-                if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, 0.0f, 0.0f);
-                continue;
-            }
-            st = row_ok(j) ? stats_of(j) : distill_careful<E, NT>(a, row, x, sh);
-        } else if (a.segs > 1)
+        const Piece p = piece_of(w, a.segs, a.seg, a.C);
+        const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
+        const float weight = a.weights ? a.weights[p.row] : 1.0f;
+        if (weight == 0.0f) {                                // ignored: 0 whatever it holds
+            if (a.segs == 1) ignored_out(a, p.row);
             continue;
-        distill_row<E, NT, true, GRAD>(a, row, x, 0, a.C, ignored, st, sh);
+        }
+        if (BUCKET) mask_listed<E, NT>(a, p.row, p.first, p.n, mask);
+        ListEntry en[2];
+        if (a.segs == 1 && threadIdx.x < WAVE) prepare_list<E>(a, p.row, x, sh, en);
+        const Running r = scan_classes<E, NT, 32 / E::VEC, false, BUCKET>(x + p.first, p.n, a.c, (const uint8_t *)mask);
+        const float3 j = block_join<NT>(r, a.c, sh);
+        if (a.segs > 1) {
+            if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, 0.0f, 0.0f);
+            continue;
+        }
+        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
+        const ListTerms t = list_terms(a, st, sh);
+        if (threadIdx.x < WAVE) loss_out(a, p.row, weight, st, t, en);
         __syncthreads();
     }
 }
 
+// The shares of a split row put together, one wave a row.
 template <class E>
-__global__ __launch_bounds__(JOIN_THREADS) void distill_join_kernel(DistillArgs a)
+__global__ __launch_bounds__(WAVE) void distill_join_kernel(DistillArgs a)
 {
-    constexpr int NT = JOIN_THREADS;
     __shared__ LogitsLds sh;
     for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        const bool ignored = a.weights && a.weights[row] == 0.0f;
-        RowStats st = {-INFINITY, -INFINITY, 0.0f};
-        if (!ignored) {
-            float3 j = make_float3(M_START, 0.0f, 0.0f);
-            for (uint32_t i = 0; i < a.segs; ++i) {
-                const float4 p = a.part[row * a.segs + i];
-                const float3 two[2] = {j, make_float3(p.x, p.y, 0.0f)};
-                j = join(two, 2, a.c);
-            }
-            st = row_ok(j) ? stats_of(j) : distill_careful<E, NT>(a, row, x, sh);
+        const float weight = a.weights ? a.weights[row] : 1.0f;
+        if (weight == 0.0f) {
+            ignored_out(a, row);
+            continue;
         }
-        distill_row<E, NT, true, false>(a, row, x, 0, a.C, ignored, st, sh);
+        ListEntry en[2];
+        float3 share = make_float3(M_START, 0.0f, 0.0f);
+        for (uint32_t i = threadIdx.x; i < a.segs; i += WAVE) {
+            const float4 p = a.part[row * a.segs + i];
+            const float3 two[2] = {share, make_float3(p.x, p.y, 0.0f)};
+            share = join(two, 2, a.c);
+        }
+        prepare_list<E>(a, row, x, sh, en);
+        const float M = wave_max(share.x);
+        const float s = wave_sum(share.y != 0.0f ? share.y * exp2_hw((share.x - M) * a.c) : 0.0f);
         __syncthreads();
+        const float3 j = make_float3(M, s, 0.0f);
+        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, WAVE>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
+        loss_out(a, row, weight, st, list_terms(a, st, sh), en);
+        __syncthreads();
+    }
+}
+
+// Losses and gradient of whole rows that fit into a block's registers: one read, one write.
+template <class E, int NT, bool BUCKET>
+__global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
+{
+    using Row = Resident<E, NT>;
+    constexpr int VEC = E::VEC;
+    __shared__ LogitsLds sh;
+    extern __shared__ uint32_t mask[];
+    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
+        typename E::raw *out = (typename E::raw *)a.grad + row * a.C;
+        const float weight = a.weights ? a.weights[row] : 1.0f;
+        if (weight == 0.0f) {
+            ignored_out(a, row);
+            zero_classes<E, NT>(out, a.C);
+            continue;
+        }
+        Row reg;
+        reg.load(x, a.C);
+        if (BUCKET) mask_listed<E, NT>(a, row, 0, a.C, mask);
+        ListEntry en[2];
+        if (threadIdx.x < WAVE) prepare_list<E>(a, row, x, sh, en);
+        Running run = running_start(a.c);
+        const uint32_t nvec = a.C / VEC;
+        reg.each(a.C, [&](int k, const float *v) {
+            if (BUCKET) {
+                float u[Row::N];
+#pragma unroll
+                for (int j = 0; j < Row::N; ++j) u[j] = v[j];
+                uint32_t b[Row::STEP], any = 0;
+#pragma unroll
+                for (int j = 0; j < Row::STEP; ++j) {
+                    const uint32_t i = (k + j) * NT + reg.tid;
+                    any |= b[j] = i < nvec ? ((const uint8_t *)mask)[i] : 0;
+                }
+                if (__any(any))
+#pragma unroll
+                    for (int j = 0; j < Row::N; ++j) u[j] = b[j / VEC] >> (j % VEC) & 1u ? -INFINITY : u[j];
+                absorb<Row::N, false>(u, a.c, run);
+            } else
+                absorb<Row::N, false>(v, a.c, run);
+        });
+        float tail = reg.tail;
+        if (BUCKET && threadIdx.x < a.C - nvec * VEC && ((const uint8_t *)mask)[nvec] >> threadIdx.x & 1u) tail = -INFINITY;
+        absorb<1, false>(&tail, a.c, run);
+        reg.forget();
+        const float3 j = block_join<NT>(run, a.c, sh);
+        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
+        const ListTerms t = list_terms(a, st, sh);
+        if (threadIdx.x < WAVE) loss_out(a, row, weight, st, t, en);
+        const float coef = weight * a.t * a.scale, dense = coef * t.dense;
+        if (t.m == -INFINITY || st.m == -INFINITY) {         // nothing has a probability, or nothing off the list
+            zero_classes<E, NT>(out, a.C);
+        } else {
+            auto value = [&](float v) { return exp2_hw((v - st.m) * a.c - st.l2) * dense; };
+#pragma unroll
+            for (int k = 0; k < Row::R; ++k) {
+                const uint32_t i = k * NT + reg.tid;
+                if (i < nvec) {
+                    float v[VEC];
+                    E::unpack(reg.w[k], v);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
+                    store_raw<E>(out + (size_t)i * VEC, E::pack(v));
+                }
+            }
+            if (threadIdx.x < a.C - nvec * VEC) out[nvec * VEC + threadIdx.x] = E::put(value(reg.tail));
+        }
+        if (t.m != -INFINITY) listed_grad<E, NT>(a, coef, t, out, a.C, 0, sh);
+        else __syncthreads();
     }
 }
 
@@ -992,14 +1232,28 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(DistillArgs a)
     __shared__ LogitsLds sh;
     const size_t work = a.rows * a.segs;
     for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
-        const size_t row = a.segs == 1 ? w : w / a.segs;
-        const uint32_t first = a.segs == 1 ? 0 : (uint32_t)(w - row * a.segs) * a.seg;
-        const uint32_t n = a.C - first < a.seg ? a.C - first : a.seg;
-        const float4 f = a.stats[row];
-        const RowStats st = {f.x, f.y, 0.0f};
-        distill_row<E, NT, false, true>(a, row, (const typename E::raw *)a.logits + row * a.stride, first, n,
-                                        a.weights && a.weights[row] == 0.0f, st, sh);
+        const Piece p = piece_of(w, a.segs, a.seg, a.C);
+        const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
+        typename E::raw *out = (typename E::raw *)a.grad + p.row * a.C + p.first;
+        const float weight = a.weights ? a.weights[p.row] : 1.0f;
+        if (weight == 0.0f) {
+            zero_classes<E, NT>(out, p.n);
+            continue;
+        }
+        ListEntry en[2];
+        if (threadIdx.x < WAVE) prepare_list<E>(a, p.row, x, sh, en);
         __syncthreads();
+        const float4 f = a.stats[p.row];
+        const RowStats st = {f.x, f.y, 0.0f};
+        const ListTerms t = list_terms(a, st, sh);
+        const float coef = weight * a.t * a.scale * (a.up ? a.up[a.up_rows ? p.row : 0] : 1.0f);
+        if (t.m == -INFINITY) {
+            zero_classes<E, NT>(out, p.n);
+            __syncthreads();
+            continue;
+        }
+        write_grad<E, NT, 16 / E::VEC, false>(st, coef * t.dense, 0.0f, x + p.first, out, p.n, a.c);
+        listed_grad<E, NT>(a, coef, t, out, p.n, p.first, sh);
     }
 }
 
@@ -1427,10 +1681,20 @@ static Split split_rows(size_t rows, uint32_t C, uint32_t blocks, uint32_t most)
     return {(C + seg - 1) / seg, seg};
 }
 constexpr uint32_t FILL_BLOCKS = 1024;
-static Split score_split(size_t rows, uint32_t C) { return split_rows(rows, C, FILL_BLOCKS, 1u << 24); }
+// What a block of NT threads holds in registers (Resident::CAP).
+static uint32_t resident(int dtype, int nt) { return 16u * nt * (dtype == ODBOX_DTYPE_F32 ? 4 : 8); }
+static Split score_split(size_t rows, uint32_t C, int k, int dtype) { return split_rows(rows, C, FILL_BLOCKS, k ? resident(dtype, 1024) : 1u << 24); }
 static Split distill_split(size_t rows, uint32_t C, int dtype)
 {
     return split_rows(rows, C, FILL_BLOCKS, (MASK_VECS - 8) * (dtype == ODBOX_DTYPE_F32 ? 4 : 8));
+}
+// f(integral_constant): the smallest block that holds n classes in registers
+template <class F>
+static void resident_variant(int dtype, uint32_t n, F f)
+{
+    if (n <= resident(dtype, 64)) f(std::integral_constant<int, 64>());
+    else if (n <= resident(dtype, 256)) f(std::integral_constant<int, 256>());
+    else f(std::integral_constant<int, 1024>());
 }
 
 #define LOGITS_LAUNCH(dtype, K_, ...)                                                       \
@@ -1479,7 +1743,7 @@ extern "C" {
 size_t odbox_label_logprobs_workspace(size_t rows, int C, int top_k)
 {
     if (C < 1 || top_k < 0) return 0;
-    const Split sp = score_split(rows, (uint32_t)C);
+    const Split sp = score_split(rows, (uint32_t)C, top_k, ODBOX_DTYPE_F32);       // (float32 has the most segments)
     return sp.segs == 1 ? 0 : rows * sp.segs * (sizeof(float4) + (size_t)top_k * sizeof(uint64_t));
 }
 
@@ -1496,7 +1760,7 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
     if (!aligned16(out_stats)) return fail(ODBOX_EINVAL, "%s: out_stats must be 16-byte aligned", name);
     if (workspace_bytes < odbox_label_logprobs_workspace(rows, C, top_k)) return fail(ODBOX_ENOSPC, "%s: workspace too small", name);
     if (!aligned16(workspace)) return fail(ODBOX_EINVAL, "%s: workspace must be 16-byte aligned", name);
-    const Split sp = score_split(rows, (uint32_t)C);
+    const Split sp = score_split(rows, (uint32_t)C, top_k, dtype);
     if (sp.segs > 1 && !workspace) return fail(ODBOX_EINVAL, "%s: NULL workspace", name);
     float4 *part = (float4 *)workspace;
     ScoreArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)top_k, LOG2E / temperature, 1.0f / temperature, labels, out_logprobs,
@@ -1511,8 +1775,12 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
         });
         return launch_status(name);
     }
-    if (top_k) LOGITS_LAUNCH(dtype, (score_kernel<E, 256, true>), grid, dim3(256), 0, st, a);
-    else LOGITS_LAUNCH(dtype, (score_kernel<E, 256, false>), grid, dim3(256), 0, st, a);
+    if (top_k)
+        resident_variant(dtype, sp.seg, [&](auto nt) {
+            constexpr int NT = decltype(nt)::value;
+            LOGITS_LAUNCH(dtype, (score_top_kernel<E, NT>), grid, dim3(NT), 0, st, a);
+        });
+    else LOGITS_LAUNCH(dtype, (score_kernel<E, 256>), grid, dim3(256), 0, st, a);
     if (sp.segs > 1) LOGITS_LAUNCH(dtype, score_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);
     return launch_status("label_logprobs");
 }
@@ -1530,7 +1798,7 @@ int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, in
     if ((uintptr_t)grad % (dtype == ODBOX_DTYPE_F32 ? 4 : 2)) return fail(ODBOX_EINVAL, "%s: grad is not aligned to its element", name);
     if (upstream_logprobs && !labels) return fail(ODBOX_EINVAL, "%s: upstream_logprobs without labels", name);
     if (upstream_top && top_k && !top_labels) return fail(ODBOX_EINVAL, "%s: upstream_top without top_labels", name);
-    const Split sp = score_split(rows, (uint32_t)C);
+    const Split sp = score_split(rows, (uint32_t)C, 0, dtype);
     ScoreGradArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)(upstream_top ? top_k : 0), LOG2E / temperature, 1.0f / temperature,
                        labels, top_labels, (const float4 *)stats, upstream_logprobs, upstream_entropy, upstream_top, grad, sp.segs, sp.seg};
     const dim3 grid = work_grid(rows * sp.segs);
@@ -1580,7 +1848,7 @@ size_t odbox_distill_loss_workspace(size_t rows, int C, int K)
     if (C < 1) return 0;
     // blocks of the sum, row losses, row statistics and shares of split rows (the smaller segments of float32)
     const Split sp = distill_split(rows, (uint32_t)C, ODBOX_DTYPE_F32);
-    return SUM_BLOCKS * sizeof(double) + ((rows + 3) / 4) * 4 * sizeof(float) + (sp.segs > 1 ? rows * (sp.segs + 1) * sizeof(float4) : 0);
+    return SUM_BLOCKS * sizeof(double) + ((rows + 3) / 4) * 4 * sizeof(float) + rows * sizeof(float4) + (sp.segs > 1 ? rows * sp.segs * sizeof(float4) : 0);
 }
 
 int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t row_stride, const float *teacher_logprobs,
@@ -1606,27 +1874,25 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
     float *per_row = out_rows ? out_rows : (float *)(partial + SUM_BLOCKS);
     const Split sp = distill_split(rows, (uint32_t)C, dtype);
     float4 *spare = (float4 *)((float *)(partial + SUM_BLOCKS) + (rows + 3) / 4 * 4);
-    float4 *keep = out_stats ? (float4 *)out_stats : sp.segs > 1 ? spare : nullptr;
+    float4 *keep = out_stats ? (float4 *)out_stats : grad ? spare : nullptr;
     DistillArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)K, LOG2E / temperature, temperature, 1.0f / temperature, scale, rest,
                      teacher_logprobs, teacher_labels, row_weights, per_row, keep, nullptr, 0, grad, sp.segs, sp.seg, spare + rows};
     const dim3 grid = work_grid(rows * sp.segs);
     const size_t lds = rest == ODBOX_REST_BUCKET ? (sp.seg / (dtype == ODBOX_DTYPE_F32 ? 4 : 8) + 8) & ~3u : 0;
-    const bool fused = grad && sp.segs == 1;
-    const bool is_short = C <= short_limit(dtype);
+    const bool is_short = C <= short_limit(dtype), fused = grad && sp.segs == 1 && (uint32_t)C <= resident(dtype, 1024);
     if (is_short) {
         distill_short(dtype, rest, grad, a, st);
-    } else if (rest == ODBOX_REST_BUCKET) {
-        if (fused) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true, true>), grid, dim3(256), lds, st, a);
-        else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true, false>), grid, dim3(256), lds, st, a);
+    } else if (fused) {
+        resident_variant(dtype, (uint32_t)C, [&](auto nt) {
+            constexpr int NT = decltype(nt)::value;
+            if (rest == ODBOX_REST_BUCKET) LOGITS_LAUNCH(dtype, (distill_fused_kernel<E, NT, true>), grid, dim3(NT), lds, st, a);
+            else LOGITS_LAUNCH(dtype, (distill_fused_kernel<E, NT, false>), grid, dim3(NT), 0, st, a);
+        });
     } else {
-        if (fused) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false, true>), grid, dim3(256), lds, st, a);
-        else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false, false>), grid, dim3(256), lds, st, a);
-    }
-    if (sp.segs > 1 && !is_short) {
-        LOGITS_LAUNCH(dtype, distill_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);
-        if (grad) {
-            LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, 256>), grid, dim3(256), 0, st, a);
-        }
+        if (rest == ODBOX_REST_BUCKET) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true>), grid, dim3(256), lds, st, a);
+        else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false>), grid, dim3(256), 0, st, a);
+        if (sp.segs > 1) LOGITS_LAUNCH(dtype, distill_join_kernel<E>, work_grid(rows), dim3(WAVE), 0, st, a);
+        if (grad) LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, 256>), grid, dim3(256), 0, st, a);
     }
     if (int rc = launch_status("distill_loss")) return rc;
     if (out_loss) {

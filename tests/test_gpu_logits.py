@@ -187,14 +187,17 @@ def check_distill(x, tl, ids, T, rest, w, losses=None, grad=None, scale=1.0, up=
     xs, t, n = _np(x), _np(tl), ids.cpu().numpy()
     ws = np.ones(len(xs)) if w is None else _np(w)
     gs = None if grad is None else _np(grad)
+    total_err = 0.0
     for i in range(len(xs)):
         loss, g, le, ge = R.distill(R.Row(xs[i], T), t[i], n[i], rest == 'bucket', ws[i])
+        total_err += le
         if losses is not None:
             R.within(_np(losses)[i], loss, le, 'loss of row %d' % i)
         if grad is not None:
             f = scale * (1.0 if up is None else float(up[i]))
             R.within(gs[i], f * g, abs(f) * (ge + 4 * R.U * np.abs(g)) + R.EPS[x.dtype] * np.abs(f * g) + R.TINY[x.dtype],
                      'gradient of row %d' % i)
+    return total_err
 
 
 @pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
@@ -212,8 +215,9 @@ def test_distill(rows, C, K, dtype, rest):
     kw = dict(temperature=T, rest=rest, row_weights=w)
     losses, grad = M.distill_loss(x, tl, ids, reduction=None, return_grad=True, **kw)
     assert losses.shape == (rows,) and losses.dtype == F32 and grad.dtype == dtype and grad.is_contiguous()
-    check_distill(x, tl, ids, T, rest, w, losses, grad)
-    assert torch.equal(losses, M.distill_loss(x, tl, ids, reduction=None, **kw))
+    err = check_distill(x, tl, ids, T, rest, w, losses, grad)
+    # without the gradient another kernel adds the row up in another order: within the same bound of the exact loss
+    check_distill(x, tl, ids, T, rest, w, M.distill_loss(x, tl, ids, reduction=None, **kw))
     # autograd: one value a row, then reduced
     xg = x.detach().requires_grad_()
     up = torch.randn(rows, generator=torch.Generator().manual_seed(6))
@@ -227,7 +231,8 @@ def test_distill(rows, C, K, dtype, rest):
         check_distill(x, tl, ids, T, rest, w, None, g1, scale=scale)
         xg = x.detach().requires_grad_()
         l2 = M.distill_loss(xg, tl, ids, reduction=reduction, **kw)
-        assert l2.item() == loss.item()
+        # both sums lie within err (the rows' bounds added) of the exact one, and each rounds once
+        assert abs(l2.item() - loss.item()) <= scale * 2 * err + 2 * R.U * abs(loss.item())
         g2, = torch.autograd.grad(3.0 * l2, xg)
         check_distill(x, tl, ids, T, rest, w, None, g2, scale=3.0 * scale)
 
