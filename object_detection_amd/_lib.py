@@ -115,6 +115,16 @@ def stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
+def raw_stream(device_index):
+    """The device's current stream as an integer.  (The Stream object that current_stream() builds costs 2.7 us.)"""
+    if _raw_stream is not None:
+        return _raw_stream(device_index)
+    return torch.cuda.current_stream(device_index).cuda_stream
+
+
 def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 

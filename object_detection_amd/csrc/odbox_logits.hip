@@ -143,7 +143,8 @@ struct LogitsLds {
     uint32_t count;
     uint32_t pick[2];
     alignas(16) int32_t id[LIST_MAX + 3];        // listed classes; -1: none, or listed before
-    float val[LIST_MAX], x[LIST_MAX];
+    float val[LIST_MAX];                         // of a listed class: its upstream value, or its q over all its entries
+    float q[ODBOX_MAX_TOP], logq[ODBOX_MAX_TOP], x[ODBOX_MAX_TOP];   // of a teacher's entry, and the student's logit there
     float sum[4];
 };
 struct TopLds {
@@ -279,47 +280,70 @@ __device__ __attribute__((noinline)) RowStats careful_stats(const typename E::ra
     return {m, l2, LN2 * (l2 - u / s)};
 }
 
-// A block's pass over n classes.  MASK: bit e of mask[v] leaves element e of vector v out.
-template <class E, int NT, int U, bool ENT, bool MASK>
-__device__ __forceinline__ Running scan_classes(const typename E::raw *x, uint32_t n, float c, const uint8_t *mask)
+// n classes of a row as seen by 16-byte loads: `head` classes up to the first boundary, nvec vectors, the rest.  Head and rest, fewer than
+// two vectors together, are the span's edge: class `edge(t)` belongs to thread t.  (Vectors across the boundaries read 25 % slower.)
+template <class E>
+struct Span {
+    uint32_t n, head, nvec, edges;
+    __device__ __forceinline__ Span(const typename E::raw *x, uint32_t count) : n(count)
+    {
+        const uint32_t gap = (uint32_t)((0u - (uint32_t)(uintptr_t)x) & 15u) / (uint32_t)sizeof(typename E::raw);
+        head = gap < n ? gap : n;
+        nvec = (n - head) / E::VEC;
+        edges = n - nvec * E::VEC;
+    }
+    __device__ __forceinline__ uint32_t edge(uint32_t t) const { return t < head ? t : t + nvec * E::VEC; }
+};
+
+// Which of a span's classes are left out: a word for every 32 values that a thread takes in one go (bit j for value j), the edge's last.
+// word(i): that of vector i (NT threads take the vectors in turn), bit(i): of its first value.
+template <class E, int NT>
+struct Mask {
+    static constexpr uint32_t VEC = E::VEC, U = 32 / E::VEC;
+    static __device__ __forceinline__ uint32_t words(uint32_t nvec) { return (nvec + U * NT - 1) / (U * NT) * NT + 1; }
+    static __device__ __forceinline__ uint32_t word(uint32_t i) { return i / (U * NT) * NT + i % NT; }
+    static __device__ __forceinline__ uint32_t bit(uint32_t i) { return i / NT % U * VEC; }
+};
+
+// A block's pass over a span.
+template <class E, int NT, bool ENT, bool MASK>
+__device__ __forceinline__ Running scan_classes(const typename E::raw *x, const Span<E> &span, float c, const uint32_t *mask)
 {
-    constexpr int VEC = E::VEC;
-    const uint32_t nvec = n / VEC;
+    constexpr int VEC = E::VEC, U = 32 / VEC;
+    using M = Mask<E, NT>;
+    const uint32_t nvec = span.nvec;
+    const typename E::raw *body = x + span.head;
     Running r = running_start(c);
     uint32_t i = threadIdx.x;
     for (; i + (U - 1) * NT < nvec; i += U * NT) {
         u32x4 w[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) w[k] = load_raw<E>(x + (size_t)(i + k * NT) * VEC);
+        for (int k = 0; k < U; ++k) w[k] = load_raw<E>(body + (size_t)(i + k * NT) * VEC);
         float v[U * VEC];
 #pragma unroll
         for (int k = 0; k < U; ++k) E::unpack(w[k], v + k * VEC);
         if (MASK) {
-            uint32_t b[U], any = 0;
+            const uint32_t b = mask[M::word(i)];
+            if (__any(b)) {
 #pragma unroll
-            for (int k = 0; k < U; ++k) any |= b[k] = mask[i + k * NT];
-            if (__any(any)) {
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) v[k * VEC + e] = b[k] >> e & 1u ? -INFINITY : v[k * VEC + e];
+                for (int j = 0; j < U * VEC; ++j) v[j] = b >> j & 1u ? -INFINITY : v[j];
             }
         }
         absorb<U * VEC, ENT>(v, c, r);
     }
     for (; i < nvec; i += NT) {
         float v[VEC];
-        E::unpack(load_raw<E>(x + (size_t)i * VEC), v);
+        E::unpack(load_raw<E>(body + (size_t)i * VEC), v);
         if (MASK) {
-            const uint32_t b = mask[i];
+            const uint32_t b = mask[M::word(i)] >> M::bit(i);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = b >> e & 1u ? -INFINITY : v[e];
         }
         absorb<VEC, ENT>(v, c, r);
     }
-    if (threadIdx.x < n - nvec * VEC) {
-        float v = E::get(x[nvec * VEC + threadIdx.x]);
-        if (MASK) v = mask[nvec] >> threadIdx.x & 1u ? -INFINITY : v;
+    if (threadIdx.x < span.edges) {
+        float v = E::get(x[span.edge(threadIdx.x)]);
+        if (MASK) v = mask[M::words(nvec) - 1] >> threadIdx.x & 1u ? -INFINITY : v;
         absorb<1, ENT>(&v, c, r);
     }
     return r;
@@ -349,17 +373,21 @@ __device__ __forceinline__ void rank_candidates(uint32_t n, uint32_t k, const To
     uint32_t sh = 0;
     while (sh < 6 && (n << (sh + 1)) <= NT) ++sh;
     const uint32_t lanes = 1u << sh, sub = threadIdx.x & (lanes - 1), step = NT >> sh;
-    for (uint32_t t0 = 0; t0 < n; t0 += step) {
-        const uint32_t t = t0 + (threadIdx.x >> sh);
-        const uint64_t mine = top.key[t < n ? t : 0];
-        uint32_t rank = 0, j = sub;
-        for (; j + 3 * lanes < n; j += 4 * lanes) {
-            const uint64_t p = top.key[j], q = top.key[j + lanes], r = top.key[j + 2 * lanes], w = top.key[j + 3 * lanes];
-            rank += (p > mine) + (q > mine) + (r > mine) + (w > mine);
+    for (uint32_t t0 = 0; t0 < n; t0 += 2 * step) {
+        const uint32_t t = t0 + (threadIdx.x >> sh), t2 = t + step;
+        const uint64_t mine = top.key[t < n ? t : 0], mine2 = top.key[t2 < n ? t2 : 0];
+        uint32_t rank = 0, rank2 = 0, j = sub;
+        for (; j + 7 * lanes < n; j += 8 * lanes) {
+            uint64_t q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = top.key[j + i * lanes];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rank += q[i] > mine, rank2 += q[i] > mine2;
         }
-        for (; j < n; j += lanes) rank += top.key[j] > mine;
-        for (uint32_t off = 1; off < lanes; off <<= 1) rank += __shfl_xor(rank, off);
+        for (; j < n; j += lanes) rank += top.key[j] > mine, rank2 += top.key[j] > mine2;
+        for (uint32_t off = 1; off < lanes; off <<= 1) rank += __shfl_xor(rank, off), rank2 += __shfl_xor(rank2, off);
         if (t < n && sub == 0 && rank < k) out(rank, mine);
+        if (t2 < n && sub == 0 && rank2 < k) out(rank2, mine2);
     }
 }
 
@@ -427,23 +455,27 @@ struct StoredKey {
 // Groups of the threshold: at least 2 k of them keep about 1.4 k candidates of values in no particular order.
 __device__ __forceinline__ uint32_t top_groups(uint32_t k) { return k <= 32 ? 64 : k <= 64 ? 128 : 256; }
 
-// A value (in f32_ordered form) that at least k of the row's classes reach and few more do: the k-th largest of G group maxima,
-// which the caller has put into top.group.
+// A value (in f32_ordered form) that at least k of the row's classes reach and few more do: the k-th largest of G group maxima in
+// top.group, its last 12 bits cleared.  One wave finds it bit by bit, counting by ballots: 20 steps of some 60 cycles, where letting
+// every group count the larger ones takes four times as long at 256 groups.
 template <int NT>
 __device__ __forceinline__ uint32_t top_threshold(uint32_t G, uint32_t k, LogitsLds &sh, TopLds &top)
 {
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    for (uint32_t t = threadIdx.x; t < G; t += NT) {
-        const uint32_t w = top.group[t];
-        uint32_t gt = 0, ge = 0;
-#pragma unroll 8
-        for (uint32_t j = 0; j < G; j += 4) {
-            const uint4 q = *(const uint4 *)&top.group[j];
-            gt += (q.x > w) + (q.y > w) + (q.z > w) + (q.w > w);
-            ge += (q.x >= w) + (q.y >= w) + (q.z >= w) + (q.w >= w);
+    if (threadIdx.x < WAVE) {
+        uint32_t g[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = (uint32_t)i * 64 < G ? top.group[i * 64 + threadIdx.x] : 0u;
+        uint32_t tau = 0;
+        for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1) {
+            const uint32_t t = tau | bit;
+            uint32_t n = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n += __popcll(__ballot(g[i] >= t));
+            if (n >= k) tau = t;
         }
-        if (gt < k && k <= ge) sh.pick[0] = w;   // one value, whoever writes it
+        if (threadIdx.x == 0) sh.pick[0] = tau;
     }
     __syncthreads();
     return sh.pick[0];
@@ -454,28 +486,27 @@ __device__ __forceinline__ void push_candidate(uint64_t key, LogitsLds &sh, TopL
     if (at < TOP_CAP) top.key[at] = key;
 }
 
-// A row, or a segment of one, in the registers of NT threads: vector i of the n / VEC whole ones at thread i % NT, one of the
-// remaining classes at each of the first threads.  What is read twice (the top classes, a gradient) is read from memory once.
+// A row, or a segment of one, in the registers of NT threads: vector i of its span at thread i % NT, one class of the edge at each of
+// the first threads.  What is read twice (the top classes, a gradient) is read from memory once.
 template <class E, int NT>
 struct Resident {
     static constexpr int R = 16, VEC = E::VEC, N = 16, STEP = N / VEC;       // N values at a time
     using raw = typename E::raw;
     u32x4 w[R];
-    float tail;
+    float edge;
     uint32_t tid;
-    static constexpr uint32_t CAP = (uint32_t)R * NT * VEC;
 
-    __device__ __forceinline__ void load(const raw *x, uint32_t n)
+    __device__ __forceinline__ void load(const raw *x, const Span<E> &span)
     {
-        const uint32_t nvec = n / VEC;
+        const raw *body = x + span.head;
         forget_thread();
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             const uint32_t i = k * NT + tid;
             w[k] = E::none();
-            if (i < nvec) w[k] = load_raw<E>(x + (size_t)i * VEC);
+            if (i < span.nvec) w[k] = load_raw<E>(body + (size_t)i * VEC);
         }
-        tail = threadIdx.x < n - nvec * VEC ? E::get(x[nvec * VEC + threadIdx.x]) : -INFINITY;
+        edge = tid < span.edges ? E::get(x[span.edge(tid)]) : -INFINITY;
     }
     // The thread's number as something new: what is computed from it (an index for every value) is not kept from row to row.
     __device__ __forceinline__ void forget_thread()
@@ -492,12 +523,11 @@ struct Resident {
     }
     // f(k, v): N values from vector k on, for the steps that hold any
     template <class F>
-    __device__ __forceinline__ void each(uint32_t n, F f) const
+    __device__ __forceinline__ void each(const Span<E> &span, F f) const
     {
-        const uint32_t nvec = n / VEC;
 #pragma unroll
         for (int k = 0; k < R; k += STEP) {
-            if ((uint32_t)k * NT < nvec) {
+            if ((uint32_t)k * NT < span.nvec) {
                 float v[N];
 #pragma unroll
                 for (int j = 0; j < STEP; ++j) E::unpack(w[k + j], v + j * VEC);
@@ -507,16 +537,19 @@ struct Resident {
     }
 };
 
-// The k best of the n classes in r, whose indices start at first; m: the thread's largest value.
-template <class E, int NT, class Out>
-__device__ __forceinline__ void top_classes(const Resident<E, NT> &r, const typename E::raw *x, uint32_t n, uint32_t first, uint32_t k, float m,
-                                            bool ok, LogitsLds &sh, TopLds &top, Out out)
+// The k best of the classes in r, whose indices start at first; m: the thread's largest value.  free_registers() is called when r is
+// no longer needed, and may load the next row into it.
+template <class E, int NT, class Free, class Out>
+__device__ __forceinline__ void top_classes(Resident<E, NT> &r, const typename E::raw *x, const Span<E> &span, uint32_t first, uint32_t k, float m,
+                                            bool ok, LogitsLds &sh, TopLds &top, Free free_registers, Out out)
 {
     using Row = Resident<E, NT>;
     constexpr int VEC = E::VEC, WAVES = NT / WAVE;
+    const uint32_t n = span.n;
     constexpr uint32_t ROOM = TOP_CAP / WAVES;
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
     bool few = false;
+    uint32_t have = 0;
     if (ok) {
         // group maxima: of neighbouring threads, or of parts of a thread's values where there are too few threads
         const uint32_t G = top_groups(k);
@@ -531,8 +564,8 @@ __device__ __forceinline__ void top_classes(const Resident<E, NT> &r, const type
             if (threadIdx.x % lanes == 0) top.group[threadIdx.x / lanes] = v;
         } else {
             // a single wave and k > 32: the values of a thread fall into four groups, or into two
-            float g[4] = {r.tail, M_START, M_START, M_START};
-            r.each(n, [&](int kk, const float *v) {
+            float g[4] = {r.edge, M_START, M_START, M_START};
+            r.each(span, [&](int kk, const float *v) {
 #pragma unroll
                 for (int j = 0; j < Resident<E, NT>::N; ++j) g[(kk + j / VEC) & 3] = vmax(g[(kk + j / VEC) & 3], v[j]);
             });
@@ -542,7 +575,6 @@ __device__ __forceinline__ void top_classes(const Resident<E, NT> &r, const type
         }
         const float tau = f32_unordered(top_threshold<NT>(G, k, sh, top));
         // candidates by wave: a ballot per value, so positions need no atomics and their order no luck
-        uint32_t have = 0;
         auto look = [&](float v, uint32_t at) {
             const uint64_t hit = __ballot(v >= tau);
             if (hit == 0) return;
@@ -551,13 +583,16 @@ __device__ __forceinline__ void top_classes(const Resident<E, NT> &r, const type
             have += __popcll(hit);
         };
         if (__any(m >= tau)) {
-            r.each(n, [&](int kk, const float *v) {
+            r.each(span, [&](int kk, const float *v) {
 #pragma unroll
-                for (int j = 0; j < Resident<E, NT>::N; ++j) look(v[j], ((kk + j / VEC) * NT + r.tid) * VEC + j % VEC);
+                for (int j = 0; j < Resident<E, NT>::N; ++j) look(v[j], span.head + ((kk + j / VEC) * NT + r.tid) * VEC + j % VEC);
             });
-            look(r.tail, n / VEC * VEC + threadIdx.x);
+            look(r.edge, span.edge(r.tid));
         }
-        // the waves' lists side by side (places beyond the row's end hold -inf, tau is M_START or more: they never count)
+    }
+    free_registers();
+    if (ok) {
+        // the waves' lists side by side (places beyond the span hold -inf, tau is M_START or more: they never count)
         const bool over = have > ROOM;
         if (WAVES > 1) {
             uint64_t mine[(ROOM + 63) / 64];
@@ -613,14 +648,19 @@ __device__ __forceinline__ float logprob_of(const ScoreArgs &a, const RowStats &
 {
     return st.m == -INFINITY ? -INFINITY : (v - st.m) * a.inv_t - LN2 * st.l2;
 }
+// The given label's logit, fetched by one thread in two steps so that neither load is waited for at the row's end.
+struct Label {
+    uint32_t id;
+    float x;
+    __device__ __forceinline__ void load_id(const ScoreArgs &a, size_t row) { id = a.logprobs && threadIdx.x == 0 ? (uint32_t)a.labels[row] : 0xffffffffu; }
+    template <class E>
+    __device__ __forceinline__ void load_logit(const ScoreArgs &a, const typename E::raw *row) { x = id < a.C ? E::get(row[id]) : 0.0f; }
+};
 template <class E>
-__device__ __forceinline__ void score_out(const ScoreArgs &a, size_t row, const typename E::raw *x, const RowStats &st)
+__device__ __forceinline__ void score_out(const ScoreArgs &a, size_t row, const Label &lab, const RowStats &st)
 {
     if (threadIdx.x != 0) return;
-    if (a.logprobs) {
-        const uint32_t lab = (uint32_t)a.labels[row];
-        a.logprobs[row] = lab < a.C ? logprob_of<E>(a, st, E::get(x[lab])) : 0.0f;
-    }
+    if (a.logprobs) a.logprobs[row] = lab.id < a.C ? logprob_of<E>(a, st, lab.x) : 0.0f;
     if (a.entropy) a.entropy[row] = st.ent;
     if (a.stats) a.stats[row] = make_float4(st.m, st.l2, st.ent, 0.0f);
 }
@@ -639,53 +679,76 @@ __device__ __forceinline__ Piece piece_of(size_t w, uint32_t segs, uint32_t seg,
 
 // Without top classes: the row streams by.
 template <class E, int NT>
-__global__ __launch_bounds__(NT) void score_kernel(ScoreArgs a)
+__global__ __launch_bounds__(NT, 8) void score_kernel(ScoreArgs a)
 {
     __shared__ LogitsLds sh;
     const size_t work = a.rows * a.segs;
     for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
         const Piece p = piece_of(w, a.segs, a.seg, a.C);
         const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
-        const Running r = scan_classes<E, NT, 32 / E::VEC, true, false>(x + p.first, p.n, a.c, nullptr);
+        Label lab;
+        if (a.segs == 1) lab.load_id(a, p.row);
+        const Running r = scan_classes<E, NT, true, false>(x + p.first, Span<E>(x + p.first, p.n), a.c, nullptr);
+        if (a.segs == 1) lab.load_logit<E>(a, x);
         const float3 j = block_join<NT>(r, a.c, sh);
         if (a.segs > 1) {
             if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, j.z, 0.0f);
             continue;
         }
-        score_out<E>(a, p.row, x, row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, 0, sh));
+        score_out<E>(a, p.row, lab, row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, 0, sh));
     }
 }
 
-// With top classes: the row stays in registers.
+// With top classes: the row stays in registers, and blocks stay for many rows: once a row's candidates are found, the next row
+// comes into the registers while they are ranked.
 template <class E, int NT>
 __global__ __launch_bounds__(NT, 4) void score_top_kernel(ScoreArgs a)
 {
     __shared__ LogitsLds sh;
     __shared__ TopLds top;
     const size_t work = a.rows * a.segs;
+    auto logits = [&](const Piece &p) { return (const typename E::raw *)a.logits + p.row * a.stride + p.first; };
+    Resident<E, NT> reg;
+    Piece p = piece_of(blockIdx.x, a.segs, a.seg, a.C);
+    Span<E> span(logits(p), p.n);
+    reg.load(logits(p), span);
     for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
-        const Piece p = piece_of(w, a.segs, a.seg, a.C);
-        const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
-        Resident<E, NT> reg;
-        reg.load(x + p.first, p.n);
+        const typename E::raw *x = logits(p);
+        Label lab;
+        if (a.segs == 1) lab.load_id(a, p.row);
         Running r = running_start(a.c);
-        reg.each(p.n, [&](int, const float *v) { absorb<Resident<E, NT>::N, true>(v, a.c, r); });
-        absorb<1, true>(&reg.tail, a.c, r);
+        reg.each(span, [&](int, const float *v) { absorb<Resident<E, NT>::N, true>(v, a.c, r); });
+        absorb<1, true>(&reg.edge, a.c, r);
+        if (a.segs == 1) lab.load_logit<E>(a, x);
         reg.forget();
         const float3 j = block_join<NT>(r, a.c, sh);
         const bool ok = row_ok(j);
+        RowStats st = {};
+        uint32_t k = a.k;
         if (a.segs > 1) {
             if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, j.z, 0.0f);
-            const uint32_t k = a.k < p.n ? a.k : p.n;        // a short last segment fills up with keys below every class's
+            k = k < p.n ? k : p.n;                           // a short last segment fills up with keys below every class's
             for (uint32_t t = k + threadIdx.x; t < a.k; t += NT) a.part_key[w * a.k + t] = 0;
-            top_classes<E, NT>(reg, x + p.first, p.n, p.first, k, r.m, ok, sh, top, [&](uint32_t rank, uint64_t key) { a.part_key[w * a.k + rank] = key; });
-            continue;
+        } else {
+            st = ok ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, 0, sh);
+            score_out<E>(a, p.row, lab, st);
         }
-        const RowStats st = ok ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, 0, sh);
-        score_out<E>(a, p.row, x, st);
-        top_classes<E, NT>(reg, x, p.n, 0, a.k, r.m, ok, sh, top, [&](uint32_t rank, uint64_t key) {
-            a.top_labels[p.row * a.k + rank] = (int32_t)top_index(key);
-            a.top_logprobs[p.row * a.k + rank] = logprob_of<E>(a, st, top_value(key));
+        const size_t row = p.row;
+        const Span<E> now = span;
+        const uint32_t first = p.first;
+        auto next_row = [&] {
+            if (w + gridDim.x >= work) return;
+            p = piece_of(w + gridDim.x, a.segs, a.seg, a.C);
+            span = Span<E>(logits(p), p.n);
+            reg.load(logits(p), span);
+        };
+        top_classes<E, NT>(reg, x, now, first, k, r.m, ok, sh, top, next_row, [&](uint32_t rank, uint64_t key) {
+            if (a.segs > 1) {
+                a.part_key[w * a.k + rank] = key;
+            } else {
+                a.top_labels[row * a.k + rank] = (int32_t)top_index(key);
+                a.top_logprobs[row * a.k + rank] = logprob_of<E>(a, st, top_value(key));
+            }
         });
     }
 }
@@ -700,59 +763,55 @@ __global__ __launch_bounds__(JOIN_THREADS) void score_join_kernel(ScoreArgs a)
     __shared__ TopLds top;
     for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        Running r = running_start(a.c);
+        // every load that depends on nothing else first
+        Label lab;
+        lab.load_id(a, row);
+        const uint32_t n = a.segs * a.k;
+        const uint64_t *keys = a.part_key + row * n;
+        const uint64_t mine = threadIdx.x < n ? keys[threadIdx.x] : 0;
+        float3 share = make_float3(M_START, 0.0f, 0.0f);     // (shares are about their exact maxima)
         for (uint32_t i = threadIdx.x; i < a.segs; i += NT) {
             const float4 p = a.part[row * a.segs + i];
-            const float3 two[2] = {make_float3(r.m, r.s, r.u), make_float3(p.x, p.y, p.z)};
-            const float3 j = join(two, 2, a.c);
-            r.m = j.x, r.s = j.y, r.u = j.z;
+            const float3 two[2] = {share, make_float3(p.x, p.y, p.z)};
+            share = join(two, 2, a.c);
         }
-        // the shares are about their exact maxima: no rounding of m c to take out, which wave_join's correction would add
-        const float M = wave_max(r.m);
-        const float D = (r.m - M) * a.c, f = exp2_hw(D);
-        const bool some = r.s != 0.0f;
-        const float3 p = make_float3(M, wave_sum(some ? r.s * f : 0.0f), wave_sum(some ? __builtin_fmaf(D, r.s, r.u) * f : 0.0f));
+        lab.load_logit<E>(a, x);
+        const float M = wave_max(share.x);
+        const float D = (share.x - M) * a.c, f = exp2_hw(D);
+        const bool some = share.y != 0.0f;
+        const float3 p = make_float3(M, wave_sum(some ? share.y * f : 0.0f), wave_sum(some ? __builtin_fmaf(D, share.y, share.z) * f : 0.0f));
         __syncthreads();
         if ((threadIdx.x & 63u) == 0) sh.part[threadIdx.x >> 6] = p;
         __syncthreads();
         const float3 j = join(sh.part, NT / WAVE, a.c);
         const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, 0, sh);
-        score_out<E>(a, row, x, st);
+        score_out<E>(a, row, lab, st);
         if (a.k) {
-            const uint32_t n = a.segs * a.k;
-            const uint64_t *keys = a.part_key + row * n;
+            uint32_t o = (uint32_t)(mine >> 24);
+            for (uint32_t i = threadIdx.x + NT; i < n; i += NT) {
+                const uint32_t q = (uint32_t)(keys[i] >> 24);
+                o = q > o ? q : o;
+            }
+            const uint32_t G = top_groups(a.k), lanes = NT / G;
+            for (uint32_t off = 1; off < lanes; off <<= 1) {
+                const uint32_t q = __shfl_xor(o, off);
+                o = q > o ? q : o;
+            }
+            __syncthreads();
+            if (threadIdx.x % lanes == 0) top.group[threadIdx.x / lanes] = o;
+            const uint32_t tau = top_threshold<NT>(G, a.k, sh, top);
+            if (threadIdx.x < n && (uint32_t)(mine >> 24) >= tau) push_candidate(mine, sh, top);
+            for (uint32_t i = threadIdx.x + NT; i < n; i += NT)
+                if ((uint32_t)(keys[i] >> 24) >= tau) push_candidate(keys[i], sh, top);
+            __syncthreads();
+            const uint32_t got = sh.count;
             auto out = [&](uint32_t rank, uint64_t key) {
                 a.top_labels[row * a.k + rank] = (int32_t)top_index(key);
                 a.top_logprobs[row * a.k + rank] = logprob_of<E>(a, st, top_value(key));
             };
-            bool few = n <= NT;
-            uint32_t got = n;
-            if (few) {
-                __syncthreads();
-                if (threadIdx.x < n) top.key[threadIdx.x] = keys[threadIdx.x];
+            if (got >= a.k && got <= TOP_CAP) {
+                rank_candidates<NT>(got, a.k, top, out);
             } else {
-                uint32_t mine = 0;
-                for (uint32_t i = threadIdx.x; i < n; i += NT) {
-                    const uint32_t o = (uint32_t)(keys[i] >> 24);
-                    mine = o > mine ? o : mine;
-                }
-                const uint32_t G = top_groups(a.k), lanes = NT / G;
-                for (uint32_t off = 1; off < lanes; off <<= 1) {
-                    const uint32_t o = __shfl_xor(mine, off);
-                    mine = o > mine ? o : mine;
-                }
-                __syncthreads();
-                if (threadIdx.x % lanes == 0) top.group[threadIdx.x / lanes] = mine;
-                const uint32_t tau = top_threshold<NT>(G, a.k, sh, top);
-                for (uint32_t i = threadIdx.x; i < n; i += NT)
-                    if ((uint32_t)(keys[i] >> 24) >= tau) push_candidate(keys[i], sh, top);
-                __syncthreads();
-                got = sh.count;
-                few = got >= a.k && got <= TOP_CAP;
-            }
-            __syncthreads();
-            if (few) rank_candidates<NT>(got, a.k, top, out);
-            else {
                 top_radix<NT>(n, a.k, sh, top, StoredKey{keys});
                 for (uint32_t t = threadIdx.x; t < a.k; t += NT) out(t, top.key[t]);
             }
@@ -799,29 +858,31 @@ __device__ __forceinline__ void write_grad(const RowStats &st, float ga, float g
         const float t = (v - st.m) * c - st.l2;
         return exp2_hw(t) * (ENT ? __builtin_fmaf(gb, vmax(t, T_FLOOR), ga) : ga);
     };
-    const uint32_t nvec = n / VEC;
+    const Span<E> span(x, n);
+    const typename E::raw *body = x + span.head;
+    typename E::raw *to = out + span.head;
     uint32_t i = threadIdx.x;
-    for (; i + (U - 1) * NT < nvec; i += U * NT) {
+    for (; i + (U - 1) * NT < span.nvec; i += U * NT) {
         u32x4 w[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) w[k] = load_raw<E>(x + (size_t)(i + k * NT) * VEC);
+        for (int k = 0; k < U; ++k) w[k] = load_raw<E>(body + (size_t)(i + k * NT) * VEC);
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             float v[VEC];
             E::unpack(w[k], v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
-            store_raw<E>(out + (size_t)(i + k * NT) * VEC, E::pack(v));
+            store_raw<E>(to + (size_t)(i + k * NT) * VEC, E::pack(v));
         }
     }
-    for (; i < nvec; i += NT) {
+    for (; i < span.nvec; i += NT) {
         float v[VEC];
-        E::unpack(load_raw<E>(x + (size_t)i * VEC), v);
+        E::unpack(load_raw<E>(body + (size_t)i * VEC), v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
-        store_raw<E>(out + (size_t)i * VEC, E::pack(v));
+        store_raw<E>(to + (size_t)i * VEC, E::pack(v));
     }
-    if (threadIdx.x < n - nvec * VEC) out[nvec * VEC + threadIdx.x] = E::put(value(E::get(x[nvec * VEC + threadIdx.x])));
+    if (threadIdx.x < span.edges) out[span.edge(threadIdx.x)] = E::put(value(E::get(x[span.edge(threadIdx.x)])));
 }
 
 struct ScoreGradArgs {
@@ -908,9 +969,31 @@ struct DistillArgs {
 // p0 nor the rest's gradient suffers the cancellation of 1 - sum p.
 //
 // Everything that needs no statistics is done by the block's first wave while the row is on its way: entries lane and lane + 64.
-struct ListEntry {
-    float q, logq, x;
-    bool on;
+struct ListEntries {
+    int32_t id[2];       // -1: an unused place
+    float t[2], x[2];
+
+    // the two loads, the second with what the first has brought
+    __device__ __forceinline__ void load_list(const DistillArgs &a, size_t row)
+    {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t j = threadIdx.x + 64 * h;
+            id[h] = -1;
+            t[h] = -INFINITY;
+            if (j < a.K) id[h] = a.ids[row * a.K + j], t[h] = a.teacher[row * a.K + j];
+        }
+    }
+    template <class E>
+    __device__ __forceinline__ void load_logits(const DistillArgs &a, const typename E::raw *row)
+    {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            x[h] = -INFINITY;
+            if ((uint32_t)id[h] < a.C) x[h] = E::get(row[id[h]]);
+            else id[h] = -1, t[h] = -INFINITY;
+        }
+    }
 };
 
 // exp(t) to about 2^-23 relative for t <= 0: the product with log2(e) in two parts
@@ -923,46 +1006,33 @@ __device__ __forceinline__ float exp_split(float t)
 }
 
 // Fills sh.id (first entries of their classes; -1 otherwise), sh.val (a class's q, summed over its entries), sh.x (the student's
-// logits there) and sh.sum: sum q, q0, and for the bucket the listed classes' maximum and sum about it.
-template <class E>
-__device__ __forceinline__ void prepare_list(const DistillArgs &a, size_t row, const typename E::raw *x, LogitsLds &sh, ListEntry (&en)[2])
+// logits there), sh.q and sh.logq (by entry) and sh.sum: sum q, q0, and for the bucket the listed classes' maximum and sum about it.
+__device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEntries &en, LogitsLds &sh)
 {
     const uint32_t lane = threadIdx.x;
-    int32_t id[2];
-    float t[2];
+    const bool on[2] = {en.id[0] >= 0, en.id[1] >= 0};
+    float q[2] = {0.0f, 0.0f}, logq[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint32_t j = lane + 64 * h;
-        id[h] = -1;
-        t[h] = -INFINITY;
-        en[h] = {0.0f, -INFINITY, -INFINITY, false};
-        if (j < a.K) {
-            id[h] = a.ids[row * a.K + j];
-            t[h] = a.teacher[row * a.K + j];
-        }
-        if ((uint32_t)id[h] < a.C) en[h].on = true, en[h].x = E::get(x[id[h]]);
-        else id[h] = -1, t[h] = -INFINITY;
-        sh.id[j] = id[h];
-    }
+    for (int h = 0; h < 2; ++h) sh.id[lane + 64 * h] = en.id[h];
     if (lane < 3) sh.id[128 + lane] = -1;
     float mass, q0 = 0.0f;
     if (!a.bucket) {
-        const float tm = wave_max(vmax(t[0], t[1]));
+        const float tm = wave_max(vmax(en.t[0], en.t[1]));
         float e[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) e[h] = en[h].on && tm > -INFINITY ? exp2_hw((t[h] - tm) * LOG2E) : 0.0f;
+        for (int h = 0; h < 2; ++h) e[h] = on[h] && tm > -INFINITY ? exp2_hw((en.t[h] - tm) * LOG2E) : 0.0f;
         const float tt = wave_sum(e[0] + e[1]), logt = LN2 * log2_hw(tt);
         mass = tm > -INFINITY ? 1.0f : 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            if (tm > -INFINITY) en[h].q = e[h] / tt, en[h].logq = (t[h] - tm) - logt;
+            if (tm > -INFINITY) q[h] = e[h] / tt, logq[h] = (en.t[h] - tm) - logt;
     } else {
         double sum = 0.0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            en[h].q = en[h].on ? exp_split(t[h]) : 0.0f;
-            en[h].logq = t[h];
-            sum += (double)en[h].q;
+            q[h] = on[h] ? exp_split(en.t[h]) : 0.0f;
+            logq[h] = en.t[h];
+            sum += (double)q[h];
         }
         for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
         const double left = 1.0 - sum;           // in double: where the list holds nearly everything, little is left of it
@@ -970,44 +1040,56 @@ __device__ __forceinline__ void prepare_list(const DistillArgs &a, size_t row, c
         mass = (float)sum;
     }
     // entries of a class listed before
-    bool first[2] = {en[0].on, en[1].on};
-    bool twice = false;
+    bool first[2] = {on[0], on[1]}, twice = false;
     for (uint32_t i = 0; i < a.K; i += 4) {
         const int4 o = *(const int4 *)&sh.id[i];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t j = lane + 64 * h;
-            if ((o.x == id[h] && i < j) || (o.y == id[h] && i + 1 < j) || (o.z == id[h] && i + 2 < j) || (o.w == id[h] && i + 3 < j)) {
+            const int32_t id = en.id[h];
+            if ((o.x == id && i < j) || (o.y == id && i + 1 < j) || (o.z == id && i + 2 < j) || (o.w == id && i + 3 < j)) {
                 twice |= first[h];
                 first[h] = false;
             }
         }
     }
-    float q[2] = {en[0].q, en[1].q};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) sh.val[lane + 64 * h] = q[h], sh.x[lane + 64 * h] = en[h].x;
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t j = lane + 64 * h;
+        sh.val[j] = sh.q[j] = q[h];
+        sh.logq[j] = logq[h];
+        sh.x[j] = en.x[h];
+    }
     if (__any(twice)) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (!first[h]) continue;
-            q[h] = 0.0f;
-            for (uint32_t i = 0; i < a.K; ++i)
-                if (sh.id[i] == id[h]) q[h] += sh.val[i];
-        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            sh.val[lane + 64 * h] = q[h];
-            if (!first[h]) sh.id[lane + 64 * h] = -1;
+            if (!first[h]) continue;
+            float sum = 0.0f;
+            for (uint32_t i = 0; i < a.K; ++i)
+                if (sh.id[i] == en.id[h]) sum += sh.q[i];
+            sh.val[lane + 64 * h] = sum;
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (!first[h]) sh.id[lane + 64 * h] = -1;
     }
     float top = -INFINITY, s = 0.0f;
     if (a.bucket) {
-        top = wave_max(vmax(first[0] ? en[0].x : -INFINITY, first[1] ? en[1].x : -INFINITY));
+        top = wave_max(vmax(first[0] ? en.x[0] : -INFINITY, first[1] ? en.x[1] : -INFINITY));
         if (top > -INFINITY)
-            s = wave_sum((first[0] ? exp2_hw((en[0].x - top) * a.c) : 0.0f) + (first[1] ? exp2_hw((en[1].x - top) * a.c) : 0.0f));
+            s = wave_sum((first[0] ? exp2_hw((en.x[0] - top) * a.c) : 0.0f) + (first[1] ? exp2_hw((en.x[1] - top) * a.c) : 0.0f));
     }
     if (lane == 0) sh.sum[0] = mass, sh.sum[1] = q0, sh.sum[2] = top, sh.sum[3] = s;
+}
+template <class E>
+__device__ __forceinline__ void load_and_prepare(const DistillArgs &a, size_t row, const typename E::raw *x, LogitsLds &sh)
+{
+    ListEntries en;
+    en.load_list(a, row);
+    en.load_logits<E>(a, x);
+    prepare_list(a, en, sh);
 }
 
 // What follows once the streamed classes' statistics are there; the same in every thread.
@@ -1038,32 +1120,35 @@ __device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, const RowS
     return r;
 }
 
-// Marks the listed classes among the n from `first` on: bit e of mask[v] for element e of vector v.
+// Marks the listed classes among a span's, which starts at class `first`.
 template <class E, int NT>
-__device__ __forceinline__ void mask_listed(const DistillArgs &a, size_t row, uint32_t first, uint32_t n, uint32_t *mask)
+__device__ __forceinline__ void mask_listed(const DistillArgs &a, size_t row, uint32_t first, const Span<E> &span, uint32_t *mask)
 {
-    constexpr int VEC = E::VEC;
-    const uint32_t words = (n / VEC + 1 + 3) / 4;
+    using M = Mask<E, NT>;
+    const uint32_t words = M::words(span.nvec);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < words; i += NT) mask[i] = 0;
+    for (uint32_t i = threadIdx.x * 4; i < words; i += NT * 4) *(uint4 *)&mask[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     for (uint32_t j = threadIdx.x; j < a.K; j += NT) {
         const uint32_t at = (uint32_t)a.ids[row * a.K + j] - first;
-        if (at < n) {
-            const uint32_t v = at / VEC, e = at % VEC;
-            atomicOr(&mask[v >> 2], 1u << ((v & 3u) * 8 + e));
-        }
+        if (at >= span.n) continue;
+        const uint32_t i = (at - span.head) / E::VEC;        // (classes of the head: far beyond nvec)
+        if (at >= span.head && i < span.nvec) atomicOr(&mask[M::word(i)], 1u << (M::bit(i) + (at - span.head) % E::VEC));
+        else atomicOr(&mask[words - 1], 1u << (at < span.head ? at : at - span.nvec * E::VEC));
     }
     __syncthreads();
 }
 
 // Loss of a row by the block's first wave.
-__device__ __forceinline__ void loss_out(const DistillArgs &a, size_t row, float w, const RowStats &st, const ListTerms &r, const ListEntry (&en)[2])
+__device__ __forceinline__ void loss_out(const DistillArgs &a, size_t row, float w, const RowStats &st, const ListTerms &r, const LogitsLds &sh)
 {
     float terms = 0.0f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-        if (en[h].q > 0.0f || en[h].q != en[h].q) terms += en[h].q * (en[h].logq - ((en[h].x - r.m) * a.inv_t - LN2 * r.l2));
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t j = threadIdx.x + 64 * h;
+        const float q = sh.q[j];
+        if (q > 0.0f || q != q) terms += q * (sh.logq[j] - ((sh.x[j] - r.m) * a.inv_t - LN2 * r.l2));
+    }
     terms = wave_sum(terms) + r.rest;
     if (threadIdx.x == 0) {
         a.out_rows[row] = r.m == -INFINITY ? 0.0f : w * a.t * a.t * terms;
@@ -1089,14 +1174,14 @@ __device__ __forceinline__ void listed_grad(const DistillArgs &a, float coef, co
     __syncthreads();
 }
 
-constexpr uint32_t MASK_VECS = 32768;            // vectors of a bucket segment: 32 KB of mask
+constexpr uint32_t MASK_CLASSES = 262144;        // of a bucket segment: 32 KB of mask
 
 // Losses, one block per row or per segment of a row: the row streams by.
 template <class E, int NT, bool BUCKET>
-__global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a)
+__global__ __launch_bounds__(NT, BUCKET ? 6 : 8) void distill_kernel(DistillArgs a)
 {
     __shared__ LogitsLds sh;
-    extern __shared__ uint32_t mask[];
+    extern __shared__ __attribute__((aligned(16))) uint32_t mask[];
     const size_t work = a.rows * a.segs;
     for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
         const Piece p = piece_of(w, a.segs, a.seg, a.C);
@@ -1106,10 +1191,10 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a)
             if (a.segs == 1) ignored_out(a, p.row);
             continue;
         }
-        if (BUCKET) mask_listed<E, NT>(a, p.row, p.first, p.n, mask);
-        ListEntry en[2];
-        if (a.segs == 1 && threadIdx.x < WAVE) prepare_list<E>(a, p.row, x, sh, en);
-        const Running r = scan_classes<E, NT, 32 / E::VEC, false, BUCKET>(x + p.first, p.n, a.c, (const uint8_t *)mask);
+        const Span<E> span(x + p.first, p.n);
+        if (BUCKET) mask_listed<E, NT>(a, p.row, p.first, span, mask);
+        if (a.segs == 1 && threadIdx.x < WAVE) load_and_prepare<E>(a, p.row, x, sh);
+        const Running r = scan_classes<E, NT, false, BUCKET>(x + p.first, span, a.c, mask);
         const float3 j = block_join<NT>(r, a.c, sh);
         if (a.segs > 1) {
             if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, 0.0f, 0.0f);
@@ -1117,7 +1202,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a)
         }
         const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
         const ListTerms t = list_terms(a, st, sh);
-        if (threadIdx.x < WAVE) loss_out(a, p.row, weight, st, t, en);
+        if (threadIdx.x < WAVE) loss_out(a, p.row, weight, st, t, sh);
         __syncthreads();
     }
 }
@@ -1134,94 +1219,113 @@ __global__ __launch_bounds__(WAVE) void distill_join_kernel(DistillArgs a)
             ignored_out(a, row);
             continue;
         }
-        ListEntry en[2];
         float3 share = make_float3(M_START, 0.0f, 0.0f);
         for (uint32_t i = threadIdx.x; i < a.segs; i += WAVE) {
             const float4 p = a.part[row * a.segs + i];
             const float3 two[2] = {share, make_float3(p.x, p.y, 0.0f)};
             share = join(two, 2, a.c);
         }
-        prepare_list<E>(a, row, x, sh, en);
+        load_and_prepare<E>(a, row, x, sh);
         const float M = wave_max(share.x);
         const float s = wave_sum(share.y != 0.0f ? share.y * exp2_hw((share.x - M) * a.c) : 0.0f);
         __syncthreads();
         const float3 j = make_float3(M, s, 0.0f);
         const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, WAVE>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
-        loss_out(a, row, weight, st, list_terms(a, st, sh), en);
+        loss_out(a, row, weight, st, list_terms(a, st, sh), sh);
         __syncthreads();
     }
 }
 
-// Losses and gradient of whole rows that fit into a block's registers: one read, one write.
+// Losses and gradient of whole rows that fit into a block's registers: one read, one write.  Blocks stay for many rows, and as
+// a vector's gradient goes out the next row's vector comes into its registers, so that memory is not idle while sums are made
+// (4096 x 131072 bfloat16: 488 us with a row after the other, XXX us like this).
 template <class E, int NT, bool BUCKET>
 __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
 {
     using Row = Resident<E, NT>;
+    using M = Mask<E, NT>;
     constexpr int VEC = E::VEC;
     __shared__ LogitsLds sh;
-    extern __shared__ uint32_t mask[];
-    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        typename E::raw *out = (typename E::raw *)a.grad + row * a.C;
-        const float weight = a.weights ? a.weights[row] : 1.0f;
-        if (weight == 0.0f) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t mask[];
+    auto logits = [&](size_t row) { return (const typename E::raw *)a.logits + row * a.stride; };
+    auto grads = [&](size_t row) { return (typename E::raw *)a.grad + row * a.C; };
+    // the next row that counts from `row` on; ignored ones are done on the way
+    auto live = [&](size_t row) {
+        for (; row < a.rows; row += gridDim.x) {
+            if (!a.weights || a.weights[row] != 0.0f) break;
             ignored_out(a, row);
-            zero_classes<E, NT>(out, a.C);
-            continue;
+            zero_classes<E, NT>(grads(row), a.C);
         }
-        Row reg;
-        reg.load(x, a.C);
-        if (BUCKET) mask_listed<E, NT>(a, row, 0, a.C, mask);
-        ListEntry en[2];
-        if (threadIdx.x < WAVE) prepare_list<E>(a, row, x, sh, en);
+        return row;
+    };
+    size_t row = live(blockIdx.x);
+    if (row >= a.rows) return;
+    Row reg;
+    ListEntries en;
+    if (threadIdx.x < WAVE) en.load_list(a, row);
+    Span<E> span(logits(row), a.C);
+    reg.load(logits(row), span);
+    while (true) {
+        const typename E::raw *x = logits(row);
+        typename E::raw *out = grads(row);
+        if (BUCKET) mask_listed<E, NT>(a, row, 0, span, mask);
+        if (threadIdx.x < WAVE) en.load_logits<E>(a, x);
         Running run = running_start(a.c);
-        const uint32_t nvec = a.C / VEC;
-        reg.each(a.C, [&](int k, const float *v) {
+        reg.each(span, [&](int k, const float *v) {
             if (BUCKET) {
+                const uint32_t b = mask[M::word(k * NT + reg.tid)] >> M::bit(k * NT);
                 float u[Row::N];
 #pragma unroll
                 for (int j = 0; j < Row::N; ++j) u[j] = v[j];
-                uint32_t b[Row::STEP], any = 0;
+                if (__any(b & ((1u << Row::N) - 1)))
 #pragma unroll
-                for (int j = 0; j < Row::STEP; ++j) {
-                    const uint32_t i = (k + j) * NT + reg.tid;
-                    any |= b[j] = i < nvec ? ((const uint8_t *)mask)[i] : 0;
-                }
-                if (__any(any))
-#pragma unroll
-                    for (int j = 0; j < Row::N; ++j) u[j] = b[j / VEC] >> (j % VEC) & 1u ? -INFINITY : u[j];
+                    for (int j = 0; j < Row::N; ++j) u[j] = b >> j & 1u ? -INFINITY : u[j];
                 absorb<Row::N, false>(u, a.c, run);
             } else
                 absorb<Row::N, false>(v, a.c, run);
         });
-        float tail = reg.tail;
-        if (BUCKET && threadIdx.x < a.C - nvec * VEC && ((const uint8_t *)mask)[nvec] >> threadIdx.x & 1u) tail = -INFINITY;
-        absorb<1, false>(&tail, a.c, run);
+        float edge = reg.edge;
+        if (BUCKET && reg.tid < span.edges && mask[M::words(span.nvec) - 1] >> reg.tid & 1u) edge = -INFINITY;
+        absorb<1, false>(&edge, a.c, run);
         reg.forget();
+        if (threadIdx.x < WAVE) prepare_list(a, en, sh);
         const float3 j = block_join<NT>(run, a.c, sh);
         const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
         const ListTerms t = list_terms(a, st, sh);
-        if (threadIdx.x < WAVE) loss_out(a, row, weight, st, t, en);
+        const float weight = a.weights ? a.weights[row] : 1.0f;
+        if (threadIdx.x < WAVE) loss_out(a, row, weight, st, t, sh);
+
+        const size_t next = live(row + gridDim.x);
+        const bool more = next < a.rows;
+        const typename E::raw *nx = logits(more ? next : row);
+        const Span<E> nspan(nx, a.C);
+        const uint32_t fetch = more ? nspan.nvec : 0;
+        if (more && threadIdx.x < WAVE) en.load_list(a, next);
         const float coef = weight * a.t * a.scale, dense = coef * t.dense;
-        if (t.m == -INFINITY || st.m == -INFINITY) {         // nothing has a probability, or nothing off the list
-            zero_classes<E, NT>(out, a.C);
-        } else {
-            auto value = [&](float v) { return exp2_hw((v - st.m) * a.c - st.l2) * dense; };
+        const bool none = t.m == -INFINITY || st.m == -INFINITY;     // nothing has a probability, or nothing off the list
+        auto value = [&](float v) { return none ? 0.0f : exp2_hw((v - st.m) * a.c - st.l2) * dense; };
+        typename E::raw *to = out + span.head;
+        if (reg.tid < span.edges) out[span.edge(reg.tid)] = E::put(value(reg.edge));
+        reg.edge = more && reg.tid < nspan.edges ? E::get(nx[nspan.edge(reg.tid)]) : -INFINITY;
 #pragma unroll
-            for (int k = 0; k < Row::R; ++k) {
-                const uint32_t i = k * NT + reg.tid;
-                if (i < nvec) {
-                    float v[VEC];
-                    E::unpack(reg.w[k], v);
+        for (int k = 0; k < Row::R; ++k) {
+            const uint32_t i = k * NT + reg.tid;
+            if (i < span.nvec) {
+                float v[VEC];
+                E::unpack(reg.w[k], v);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
-                    store_raw<E>(out + (size_t)i * VEC, E::pack(v));
-                }
+                for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
+                store_raw<E>(to + (size_t)i * VEC, E::pack(v));
             }
-            if (threadIdx.x < a.C - nvec * VEC) out[nvec * VEC + threadIdx.x] = E::put(value(reg.tail));
+            reg.w[k] = E::none();
+            if (i < fetch) reg.w[k] = load_raw<E>(nx + nspan.head + (size_t)i * VEC);
         }
         if (t.m != -INFINITY) listed_grad<E, NT>(a, coef, t, out, a.C, 0, sh);
         else __syncthreads();
+        if (!more) break;
+        row = next;
+        span = nspan;
+        reg.forget_thread();
     }
 }
 
@@ -1240,8 +1344,7 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(DistillArgs a)
             zero_classes<E, NT>(out, p.n);
             continue;
         }
-        ListEntry en[2];
-        if (threadIdx.x < WAVE) prepare_list<E>(a, p.row, x, sh, en);
+        if (threadIdx.x < WAVE) load_and_prepare<E>(a, p.row, x, sh);
         __syncthreads();
         const float4 f = a.stats[p.row];
         const RowStats st = {f.x, f.y, 0.0f};
@@ -1289,11 +1392,17 @@ __device__ __forceinline__ float group_sum(float x)
     if (L >= 64) x += __shfl_xor(x, 32);
     return x;
 }
-template <int L, class T>
-__device__ __forceinline__ T group_fold(T x, T (*op)(T, T))
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false); }
+template <int L, class Op>
+__device__ __forceinline__ uint32_t group_fold(uint32_t x, Op op)
 {
-#pragma unroll
-    for (int off = 1; off < L; off <<= 1) x = op(x, (T)__shfl_xor(x, off));
+    x = op(x, dpp_u<0xB1>(x));
+    x = op(x, dpp_u<0x4E>(x));
+    if (L >= 8) x = op(x, dpp_u<0x141>(x));
+    if (L >= 16) x = op(x, dpp_u<0x140>(x));
+    if (L >= 64) x = op(x, (uint32_t)__shfl_xor(x, 16));
+    if (L >= 64) x = op(x, (uint32_t)__shfl_xor(x, 32));
     return x;
 }
 
@@ -1414,11 +1523,11 @@ __global__ __launch_bounds__(SHORT_THREADS) void score_short_kernel(ScoreArgs a)
             uint32_t best = 0;
 #pragma unroll
             for (int i = 0; i < Row::PV; ++i) best = o[i] > best ? o[i] : best;
-            best = group_fold<L, uint32_t>(best, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
+            best = group_fold<L>(best, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
             uint32_t win = 0xffffffffu;
 #pragma unroll
             for (int i = Row::PV - 1; i >= 0; --i) win = o[i] == best ? r.base(i / Row::VEC) + i % Row::VEC : win;
-            win = group_fold<L, uint32_t>(win, [](uint32_t p, uint32_t q) { return p < q ? p : q; });
+            win = group_fold<L>(win, [](uint32_t p, uint32_t q) { return p < q ? p : q; });
 #pragma unroll
             for (int i = 0; i < Row::PV; ++i) o[i] = win - r.base(i / Row::VEC) == (uint32_t)(i % Row::VEC) ? 0u : o[i];
             if (round % L == r.lane) {
@@ -1487,7 +1596,7 @@ __global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArg
     using Row = ShortRow<E, L, S>;
     constexpr uint32_t RB = SHORT_THREADS / L;
     constexpr bool LISTED = BUCKET || GRAD;                  // the LDS is needed
-    extern __shared__ float listed[];
+    extern __shared__ __attribute__((aligned(16))) float listed[];
     const uint32_t pitch = (a.C + 3) & ~3u;
     float *list = listed + (LISTED ? (threadIdx.x / L) * pitch : 0);
     for (size_t row = (size_t)blockIdx.x * RB + threadIdx.x / L; row < a.rows; row += (size_t)gridDim.x * RB) {
@@ -1528,7 +1637,7 @@ __global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArg
                 else twice = true;
             }
             fence();
-            twice = group_fold<L, int>(twice, [](int p, int q) { return p | q; }) != 0;
+            twice = group_fold<L>(twice ? 1u : 0u, [](uint32_t p, uint32_t q) { return p | q; }) != 0;
         }
         auto off_list = [&](int k, int e) { return list[r.base(k) + e] < 0.0f; };
         RowStats st;
@@ -1681,12 +1790,19 @@ static Split split_rows(size_t rows, uint32_t C, uint32_t blocks, uint32_t most)
     return {(C + seg - 1) / seg, seg};
 }
 constexpr uint32_t FILL_BLOCKS = 1024;
-// What a block of NT threads holds in registers (Resident::CAP).
+static uint32_t fuse_rows() { const char *e = getenv("LG_FUSE"); return e ? atoi(e) : 512; }
+// What a block of NT threads holds in registers.
 static uint32_t resident(int dtype, int nt) { return 16u * nt * (dtype == ODBOX_DTYPE_F32 ? 4 : 8); }
 static Split score_split(size_t rows, uint32_t C, int k, int dtype) { return split_rows(rows, C, FILL_BLOCKS, k ? resident(dtype, 1024) : 1u << 24); }
-static Split distill_split(size_t rows, uint32_t C, int dtype)
+static Split distill_split(size_t rows, uint32_t C)
 {
-    return split_rows(rows, C, FILL_BLOCKS, (MASK_VECS - 8) * (dtype == ODBOX_DTYPE_F32 ? 4 : 8));
+    return split_rows(rows, C, FILL_BLOCKS, MASK_CLASSES);
+}
+// Blocks that stay: as many as the 256 CUs hold at four waves a SIMD (128 registers).
+static dim3 staying_grid(size_t work, int nt)
+{
+    const size_t fit = 256 * (1024 / nt);
+    return dim3((uint32_t)(work < fit ? work : fit));
 }
 // f(integral_constant): the smallest block that holds n classes in registers
 template <class F>
@@ -1778,7 +1894,7 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
     if (top_k)
         resident_variant(dtype, sp.seg, [&](auto nt) {
             constexpr int NT = decltype(nt)::value;
-            LOGITS_LAUNCH(dtype, (score_top_kernel<E, NT>), grid, dim3(NT), 0, st, a);
+            LOGITS_LAUNCH(dtype, (score_top_kernel<E, NT>), staying_grid(rows * sp.segs, NT), dim3(NT), 0, st, a);
         });
     else LOGITS_LAUNCH(dtype, (score_kernel<E, 256>), grid, dim3(256), 0, st, a);
     if (sp.segs > 1) LOGITS_LAUNCH(dtype, score_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);
@@ -1846,8 +1962,8 @@ size_t odbox_distill_loss_workspace(size_t rows, int C, int K)
 {
     (void)K;
     if (C < 1) return 0;
-    // blocks of the sum, row losses, row statistics and shares of split rows (the smaller segments of float32)
-    const Split sp = distill_split(rows, (uint32_t)C, ODBOX_DTYPE_F32);
+    // blocks of the sum, row losses, row statistics and shares of split rows
+    const Split sp = distill_split(rows, (uint32_t)C);
     return SUM_BLOCKS * sizeof(double) + ((rows + 3) / 4) * 4 * sizeof(float) + rows * sizeof(float4) + (sp.segs > 1 ? rows * sp.segs * sizeof(float4) : 0);
 }
 
@@ -1872,24 +1988,26 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
     if (!workspace) return fail(ODBOX_EINVAL, "%s: NULL workspace", name);
     double *partial = (double *)workspace;
     float *per_row = out_rows ? out_rows : (float *)(partial + SUM_BLOCKS);
-    const Split sp = distill_split(rows, (uint32_t)C, dtype);
+    const bool is_short = C <= short_limit(dtype);
+    const bool fused = grad && !is_short && rows >= fuse_rows() && (uint32_t)C <= resident(dtype, 1024);
+    const Split sp = fused ? Split{1, (uint32_t)C} : distill_split(rows, (uint32_t)C);
     float4 *spare = (float4 *)((float *)(partial + SUM_BLOCKS) + (rows + 3) / 4 * 4);
     float4 *keep = out_stats ? (float4 *)out_stats : grad ? spare : nullptr;
     DistillArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)K, LOG2E / temperature, temperature, 1.0f / temperature, scale, rest,
                      teacher_logprobs, teacher_labels, row_weights, per_row, keep, nullptr, 0, grad, sp.segs, sp.seg, spare + rows};
     const dim3 grid = work_grid(rows * sp.segs);
-    const size_t lds = rest == ODBOX_REST_BUCKET ? (sp.seg / (dtype == ODBOX_DTYPE_F32 ? 4 : 8) + 8) & ~3u : 0;
-    const bool is_short = C <= short_limit(dtype), fused = grad && sp.segs == 1 && (uint32_t)C <= resident(dtype, 1024);
+    // Mask::words for NT threads, and what clearing them by fours may add
+    const auto mask_bytes = [&](uint32_t nt) { return rest == ODBOX_REST_BUCKET ? ((size_t)(sp.seg + 32 * nt - 1) / (32 * nt) * nt + 4) * 4 : 0; };
     if (is_short) {
         distill_short(dtype, rest, grad, a, st);
     } else if (fused) {
         resident_variant(dtype, (uint32_t)C, [&](auto nt) {
             constexpr int NT = decltype(nt)::value;
-            if (rest == ODBOX_REST_BUCKET) LOGITS_LAUNCH(dtype, (distill_fused_kernel<E, NT, true>), grid, dim3(NT), lds, st, a);
-            else LOGITS_LAUNCH(dtype, (distill_fused_kernel<E, NT, false>), grid, dim3(NT), 0, st, a);
+            if (rest == ODBOX_REST_BUCKET) LOGITS_LAUNCH(dtype, (distill_fused_kernel<E, NT, true>), staying_grid(rows, NT), dim3(NT), mask_bytes(NT), st, a);
+            else LOGITS_LAUNCH(dtype, (distill_fused_kernel<E, NT, false>), staying_grid(rows, NT), dim3(NT), 0, st, a);
         });
     } else {
-        if (rest == ODBOX_REST_BUCKET) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true>), grid, dim3(256), lds, st, a);
+        if (rest == ODBOX_REST_BUCKET) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true>), grid, dim3(256), mask_bytes(256), st, a);
         else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false>), grid, dim3(256), 0, st, a);
         if (sp.segs > 1) LOGITS_LAUNCH(dtype, distill_join_kernel<E>, work_grid(rows), dim3(WAVE), 0, st, a);
         if (grad) LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, 256>), grid, dim3(256), 0, st, a);
@@ -1917,7 +2035,7 @@ int odbox_distill_loss_backward(const void *logits, int dtype, size_t rows, int 
     if (rows == 0) return 0;
     if (!stats || !upstream || !grad) return fail(ODBOX_EINVAL, "%s: NULL stats, upstream or grad", name);
     if (!aligned16(stats)) return fail(ODBOX_EINVAL, "%s: stats must be 16-byte aligned", name);
-    const Split sp = distill_split(rows, (uint32_t)C, dtype);
+    const Split sp = distill_split(rows, (uint32_t)C);
     DistillArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)K, LOG2E / temperature, temperature, 1.0f / temperature, scale, rest, teacher_logprobs,
                      teacher_labels, row_weights, nullptr, (float4 *)stats, upstream, upstream_rows, grad, sp.segs, sp.seg, nullptr};
     if (C <= short_limit(dtype)) {

@@ -134,20 +134,21 @@ def _logits(x):
     """Logits on their own GPU (host data: on the current one) in float32 / float16 / bfloat16; other types become float32."""
     if not isinstance(x, torch.Tensor):
         x = torch.as_tensor(x)
-    dev = x.device if x.is_cuda else _lib.require_gpu()
-    x = x.to(device=dev, dtype=x.dtype if x.dtype in _DTYPE_CODE else torch.float32, non_blocking=True)
+    if not (x.is_cuda and x.dtype in _DTYPE_CODE):
+        dev = x.device if x.is_cuda else _lib.require_gpu()
+        x = x.to(device=dev, dtype=x.dtype if x.dtype in _DTYPE_CODE else torch.float32, non_blocking=True)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_LOGITS:
         raise ValueError('logits %r: the last axis holds 1..%d classes' % (tuple(x.shape), MAX_LOGITS))
     return x
 
 
 def _rows_view(x):
-    """[..., C] -> ([rows, C] view, rows, C, elements between rows).  The classes of a row have to lie side by side and the
-    rows evenly apart (a padded vocabulary, an expanded row): anything else is copied once."""
-    C = int(x.shape[-1])
+    """[..., C] -> (tensor whose storage is read, rows, C, elements between rows).  The classes of a row have to lie side by side
+    and the rows evenly apart (a padded vocabulary, an expanded row): anything else is copied once."""
+    C = x.shape[-1]
     rows = x.numel() // C
-    if rows == 0:
-        return x.reshape(0, C), 0, C, C
+    if x.is_contiguous() or rows == 0:
+        return x, rows, C, C
     if x.dim() == 1:
         x = x.unsqueeze(0)
     if C > 1 and x.stride(-1) != 1:
@@ -156,15 +157,17 @@ def _rows_view(x):
         v = x.view(rows, C)
     except RuntimeError:
         v = x.contiguous().view(rows, C)
-    return v, rows, C, (int(v.stride(0)) if rows > 1 else C)
+    return v, rows, C, (v.stride(0) if rows > 1 else C)
 
 
 def _side(x, dtype, device, shape, what):
     """A tensor that goes with the rows of the logits, contiguous on their device."""
     if not isinstance(x, torch.Tensor):
         x = torch.as_tensor(x)
-    if tuple(x.shape) != tuple(shape):
+    if x.shape != shape:
         raise ValueError('%s %r does not fit the logits: expected %r' % (what, tuple(x.shape), tuple(shape)))
+    if x.dtype == dtype and x.device == device and x.is_contiguous() and not x.requires_grad:
+        return x
     return x.detach().to(device=device, dtype=dtype, non_blocking=True).contiguous()
 
 
@@ -175,9 +178,16 @@ def _temperature(t):
     return t
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """Launches go to the logits' device and its current stream, whichever device is current."""
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else _HERE
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 class LabelLogprobs(typing.NamedTuple):
@@ -191,23 +201,37 @@ class LabelLogprobs(typing.NamedTuple):
 def _score_launch(x, labels, top_k, temperature, want_stats):
     lib = _lib.load()
     v, rows, C, stride = _rows_view(x)
-    lead = x.shape[:-1]
-    new = dict(dtype=torch.float32, device=x.device)
-    ent = torch.empty(lead, **new)
-    lp = torch.empty(lead, **new) if labels is not None else None
-    tlp = torch.empty(lead + (top_k,), **new) if top_k else None
-    tid = torch.empty(lead + (top_k,), dtype=torch.int32, device=x.device) if top_k else None
-    stats = torch.empty((rows, 4), **new) if want_stats else None
+    lead, dev = x.shape[:-1], x.device
+    ent = torch.empty(lead, dtype=torch.float32, device=dev)
+    lp = torch.empty_like(ent) if labels is not None else None
+    tlp = tid = None
+    if top_k:
+        tlp = torch.empty(lead + (top_k,), dtype=torch.float32, device=dev)
+        tid = torch.empty_like(tlp, dtype=torch.int32)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
     need = lib.odbox_label_logprobs_workspace(rows, C, top_k)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _lib.check(lib.odbox_label_logprobs(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _lib.ptr(labels), top_k, temperature,
-                                        _lib.ptr(lp), _lib.ptr(ent), _lib.ptr(tlp), _lib.ptr(tid), _lib.ptr(stats),
-                                        _lib.ptr(ws), need, _lib.stream_ptr()), 'odbox_label_logprobs')
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rc = lib.odbox_label_logprobs(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _ptr(labels), top_k, temperature, _ptr(lp),
+                                  ent.data_ptr(), _ptr(tlp), _ptr(tid), _ptr(stats), _ptr(ws), need, _lib.raw_stream(dev.index))
+    if rc:
+        _lib.check(rc, 'odbox_label_logprobs')
     return lp, ent, tlp, tid, stats
 
 
 def _upstream(g, device):
-    return None if g is None else g.detach().to(device=device, dtype=torch.float32).contiguous()
+    if g is None or (g.dtype == torch.float32 and g.device == device and g.is_contiguous()):
+        return g
+    return g.detach().to(device=device, dtype=torch.float32).contiguous()
+
+
+def _backward(launch):
+    """launch(ctx, *grads) as a Function's backward.  The gradient itself has no derivative; the decorator that says so costs
+    more than the launch, and only a backward pass that is recorded (create_graph) needs it."""
+    once = once_differentiable(launch)
+
+    def backward(ctx, *grads):
+        return (once if torch.is_grad_enabled() else launch)(ctx, *grads)
+    return staticmethod(backward)
 
 
 class _LabelLogprobsFn(torch.autograd.Function):
@@ -224,22 +248,22 @@ class _LabelLogprobsFn(torch.autograd.Function):
             ctx.mark_non_differentiable(tid)
         return lp, ent, tlp, tid
 
-    @staticmethod
-    @once_differentiable
+    @_backward
     def backward(ctx, g_lp, g_ent, g_top, _g_id):
-        x, labels, tid, stats = ctx.saved_tensors
-        top_k, temperature = ctx.cfg
         if g_lp is None and g_ent is None and g_top is None:
             return None, None, None, None
-        lib = _lib.load()
-        with _on(x.device):
+        x, labels, tid, stats = ctx.saved_tensors
+        top_k, temperature = ctx.cfg
+        dev = x.device
+        with _on(dev):
             v, rows, C, stride = _rows_view(x)
-            g_lp, g_ent, g_top = (_upstream(g, x.device) for g in (g_lp, g_ent, g_top))
-            grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            _lib.check(lib.odbox_label_logprobs_backward(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _lib.ptr(labels), top_k,
-                                                         _lib.ptr(tid), temperature, _lib.ptr(stats), _lib.ptr(g_lp), _lib.ptr(g_ent),
-                                                         _lib.ptr(g_top), _lib.ptr(grad), _lib.stream_ptr()),
-                       'odbox_label_logprobs_backward')
+            g_lp, g_ent, g_top = _upstream(g_lp, dev), _upstream(g_ent, dev), _upstream(g_top, dev)
+            grad = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            rc = _lib.load().odbox_label_logprobs_backward(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _ptr(labels), top_k, _ptr(tid),
+                                                           temperature, stats.data_ptr(), _ptr(g_lp), _ptr(g_ent), _ptr(g_top),
+                                                           grad.data_ptr(), _lib.raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, 'odbox_label_logprobs_backward')
         return grad, None, None, None
 
 
@@ -273,17 +297,18 @@ def _distill_launch(x, tl, ids, w, cfg, per_row, want_stats, want_grad):
     lib = _lib.load()
     temperature, rest, scale = cfg
     v, rows, C, stride = _rows_view(x)
-    K = int(ids.shape[-1])
-    new = dict(dtype=torch.float32, device=x.device)
-    out = torch.empty(x.shape[:-1] if per_row else (), **new)
-    stats = torch.empty((rows, 4), **new) if want_stats else None
-    grad = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_grad else None
+    K, dev = ids.shape[-1], x.device
+    out = torch.empty(x.shape[:-1] if per_row else (), dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
+    grad = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_grad else None
     need = lib.odbox_distill_loss_workspace(rows, C, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    _lib.check(lib.odbox_distill_loss(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _lib.ptr(tl), _lib.ptr(ids), K, temperature,
-                                      rest, _lib.ptr(w), scale, _lib.ptr(out) if per_row else None,
-                                      None if per_row else _lib.ptr(out), _lib.ptr(stats), _lib.ptr(grad), _lib.ptr(ws), need,
-                                      _lib.stream_ptr()), 'odbox_distill_loss')
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    to = out.data_ptr()
+    rc = lib.odbox_distill_loss(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, tl.data_ptr(), ids.data_ptr(), K, temperature, rest,
+                                _ptr(w), scale, to if per_row else None, None if per_row else to, _ptr(stats), _ptr(grad),
+                                ws.data_ptr(), need, _lib.raw_stream(dev.index))
+    if rc:
+        _lib.check(rc, 'odbox_distill_loss')
     return out, stats, grad
 
 
@@ -299,20 +324,20 @@ class _DistillLossFn(torch.autograd.Function):
         ctx.cfg, ctx.per_row = cfg, per_row
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_backward
     def backward(ctx, g):
         x, tl, ids, w, stats = ctx.saved_tensors
         temperature, rest, scale = ctx.cfg
-        lib = _lib.load()
-        with _on(x.device):
+        dev = x.device
+        with _on(dev):
             v, rows, C, stride = _rows_view(x)
-            g = _upstream(g, x.device)
-            grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            _lib.check(lib.odbox_distill_loss_backward(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, _lib.ptr(tl), _lib.ptr(ids),
-                                                       int(ids.shape[-1]), temperature, rest, _lib.ptr(w), scale, _lib.ptr(stats),
-                                                       _lib.ptr(g), int(ctx.per_row), _lib.ptr(grad), _lib.stream_ptr()),
-                       'odbox_distill_loss_backward')
+            g = _upstream(g, dev)
+            grad = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            rc = _lib.load().odbox_distill_loss_backward(v.data_ptr(), _DTYPE_CODE[x.dtype], rows, C, stride, tl.data_ptr(), ids.data_ptr(),
+                                                         ids.shape[-1], temperature, rest, _ptr(w), scale, stats.data_ptr(), g.data_ptr(),
+                                                         int(ctx.per_row), grad.data_ptr(), _lib.raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, 'odbox_distill_loss_backward')
         return grad, None, None, None, None, None
 
 
@@ -339,7 +364,7 @@ def distill_loss(logits, teacher_logprobs, teacher_labels, temperature: float = 
         raise ValueError("rest %r is neither 'renormalise' nor 'bucket'" % (rest,))
     if not isinstance(teacher_labels, torch.Tensor):
         teacher_labels = torch.as_tensor(teacher_labels)
-    lead = tuple(x.shape[:-1])
+    lead = x.shape[:-1]
     K = int(teacher_labels.shape[-1]) if teacher_labels.dim() else 0
     if not 1 <= K <= MAX_TOP:
         raise ValueError('teacher_labels %r: the last axis holds 1..%d classes' % (tuple(teacher_labels.shape), MAX_TOP))
