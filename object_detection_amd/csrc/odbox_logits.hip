@@ -87,17 +87,19 @@ struct BF16 {
         return __builtin_bit_cast(u32x4, __builtin_convertvector(f, bf16x8));
     }
 };
-template <class E>
+// PASSING: data that passes by once goes around the caches.
+template <class E, bool PASSING = false>
 __device__ __forceinline__ u32x4 load_raw(const typename E::raw *p)
 {
     typedef typename Unaligned<u32x4, sizeof(typename E::raw)>::type mem;
-    return *(const mem *)p;
+    return PASSING ? __builtin_nontemporal_load((const mem *)p) : *(const mem *)p;
 }
-template <class E>
+template <class E, bool PASSING = false>
 __device__ __forceinline__ void store_raw(typename E::raw *p, u32x4 v)
 {
     typedef typename Unaligned<u32x4, sizeof(typename E::raw)>::type mem;
-    *(mem *)p = v;
+    if (PASSING) __builtin_nontemporal_store(v, (mem *)p);
+    else *(mem *)p = v;
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -306,7 +308,7 @@ struct Mask {
 };
 
 // A block's pass over a span.
-template <class E, int NT, bool ENT, bool MASK>
+template <class E, int NT, bool ENT, bool MASK, bool PASSING>
 __device__ __forceinline__ Running scan_classes(const typename E::raw *x, const Span<E> &span, float c, const uint32_t *mask)
 {
     constexpr int VEC = E::VEC, U = 32 / VEC;
@@ -318,7 +320,7 @@ __device__ __forceinline__ Running scan_classes(const typename E::raw *x, const 
     for (; i + (U - 1) * NT < nvec; i += U * NT) {
         u32x4 w[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) w[k] = load_raw<E>(body + (size_t)(i + k * NT) * VEC);
+        for (int k = 0; k < U; ++k) w[k] = load_raw<E, PASSING>(body + (size_t)(i + k * NT) * VEC);
         float v[U * VEC];
 #pragma unroll
         for (int k = 0; k < U; ++k) E::unpack(w[k], v + k * VEC);
@@ -333,7 +335,7 @@ __device__ __forceinline__ Running scan_classes(const typename E::raw *x, const 
     }
     for (; i < nvec; i += NT) {
         float v[VEC];
-        E::unpack(load_raw<E>(body + (size_t)i * VEC), v);
+        E::unpack(load_raw<E, PASSING>(body + (size_t)i * VEC), v);
         if (MASK) {
             const uint32_t b = mask[M::word(i)] >> M::bit(i);
 #pragma unroll
@@ -496,6 +498,7 @@ struct Resident {
     float edge;
     uint32_t tid;
 
+    template <bool PASSING>
     __device__ __forceinline__ void load(const raw *x, const Span<E> &span)
     {
         const raw *body = x + span.head;
@@ -504,7 +507,7 @@ struct Resident {
         for (int k = 0; k < R; ++k) {
             const uint32_t i = k * NT + tid;
             w[k] = E::none();
-            if (i < span.nvec) w[k] = load_raw<E>(body + (size_t)i * VEC);
+            if (i < span.nvec) w[k] = load_raw<E, PASSING>(body + (size_t)i * VEC);
         }
         edge = tid < span.edges ? E::get(x[span.edge(tid)]) : -INFINITY;
     }
@@ -678,7 +681,7 @@ __device__ __forceinline__ Piece piece_of(size_t w, uint32_t segs, uint32_t seg,
 }
 
 // Without top classes: the row streams by.
-template <class E, int NT>
+template <class E, int NT, bool PASSING>
 __global__ __launch_bounds__(NT, 8) void score_kernel(ScoreArgs a)
 {
     __shared__ LogitsLds sh;
@@ -688,7 +691,7 @@ __global__ __launch_bounds__(NT, 8) void score_kernel(ScoreArgs a)
         const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
         Label lab;
         if (a.segs == 1) lab.load_id(a, p.row);
-        const Running r = scan_classes<E, NT, true, false>(x + p.first, Span<E>(x + p.first, p.n), a.c, nullptr);
+        const Running r = scan_classes<E, NT, true, false, PASSING>(x + p.first, Span<E>(x + p.first, p.n), a.c, nullptr);
         if (a.segs == 1) lab.load_logit<E>(a, x);
         const float3 j = block_join<NT>(r, a.c, sh);
         if (a.segs > 1) {
@@ -711,7 +714,7 @@ __global__ __launch_bounds__(NT, 4) void score_top_kernel(ScoreArgs a)
     Resident<E, NT> reg;
     Piece p = piece_of(blockIdx.x, a.segs, a.seg, a.C);
     Span<E> span(logits(p), p.n);
-    reg.load(logits(p), span);
+    reg.template load<false>(logits(p), span);
     for (size_t w = blockIdx.x; w < work; w += gridDim.x) {
         const typename E::raw *x = logits(p);
         Label lab;
@@ -740,7 +743,7 @@ __global__ __launch_bounds__(NT, 4) void score_top_kernel(ScoreArgs a)
             if (w + gridDim.x >= work) return;
             p = piece_of(w + gridDim.x, a.segs, a.seg, a.C);
             span = Span<E>(logits(p), p.n);
-            reg.load(logits(p), span);
+            reg.template load<false>(logits(p), span);
         };
         top_classes<E, NT>(reg, x, now, first, k, r.m, ok, sh, top, next_row, [&](uint32_t rank, uint64_t key) {
             if (a.segs > 1) {
@@ -865,22 +868,22 @@ __device__ __forceinline__ void write_grad(const RowStats &st, float ga, float g
     for (; i + (U - 1) * NT < span.nvec; i += U * NT) {
         u32x4 w[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) w[k] = load_raw<E>(body + (size_t)(i + k * NT) * VEC);
+        for (int k = 0; k < U; ++k) w[k] = load_raw<E, true>(body + (size_t)(i + k * NT) * VEC);
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             float v[VEC];
             E::unpack(w[k], v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
-            store_raw<E>(to + (size_t)(i + k * NT) * VEC, E::pack(v));
+            store_raw<E, true>(to + (size_t)(i + k * NT) * VEC, E::pack(v));
         }
     }
     for (; i < span.nvec; i += NT) {
         float v[VEC];
-        E::unpack(load_raw<E>(body + (size_t)i * VEC), v);
+        E::unpack(load_raw<E, true>(body + (size_t)i * VEC), v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
-        store_raw<E>(to + (size_t)i * VEC, E::pack(v));
+        store_raw<E, true>(to + (size_t)i * VEC, E::pack(v));
     }
     if (threadIdx.x < span.edges) out[span.edge(threadIdx.x)] = E::put(value(E::get(x[span.edge(threadIdx.x)])));
 }
@@ -1177,7 +1180,7 @@ __device__ __forceinline__ void listed_grad(const DistillArgs &a, float coef, co
 constexpr uint32_t MASK_CLASSES = 262144;        // of a bucket segment: 32 KB of mask
 
 // Losses, one block per row or per segment of a row: the row streams by.
-template <class E, int NT, bool BUCKET>
+template <class E, int NT, bool BUCKET, bool PASSING>
 __global__ __launch_bounds__(NT, BUCKET ? 6 : 8) void distill_kernel(DistillArgs a)
 {
     __shared__ LogitsLds sh;
@@ -1194,7 +1197,7 @@ __global__ __launch_bounds__(NT, BUCKET ? 6 : 8) void distill_kernel(DistillArgs
         const Span<E> span(x + p.first, p.n);
         if (BUCKET) mask_listed<E, NT>(a, p.row, p.first, span, mask);
         if (a.segs == 1 && threadIdx.x < WAVE) load_and_prepare<E>(a, p.row, x, sh);
-        const Running r = scan_classes<E, NT, false, BUCKET>(x + p.first, span, a.c, mask);
+        const Running r = scan_classes<E, NT, false, BUCKET, PASSING>(x + p.first, span, a.c, mask);
         const float3 j = block_join<NT>(r, a.c, sh);
         if (a.segs > 1) {
             if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, 0.0f, 0.0f);
@@ -1236,9 +1239,9 @@ __global__ __launch_bounds__(WAVE) void distill_join_kernel(DistillArgs a)
     }
 }
 
-// Losses and gradient of whole rows that fit into a block's registers: one read, one write.  Blocks stay for many rows, and as
-// a vector's gradient goes out the next row's vector comes into its registers, so that memory is not idle while sums are made
-// (4096 x 131072 bfloat16: 488 us with a row after the other, XXX us like this).
+// Losses and gradient of whole rows that fit into a block's registers: one read, one write.  (Fetching the next row's vectors as this
+// row's gradients leave them was measured too: 4096 x 131072 bfloat16 433 -> 476 us.  Memory moves reads and writes faster apart.)
+// Reads go around the caches, and writes where rows are long: 444 -> 431 us, 1024 rows 142 -> 128, 4096 x 30000 120 -> 104.
 template <class E, int NT, bool BUCKET>
 __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
 {
@@ -1247,27 +1250,20 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
     constexpr int VEC = E::VEC;
     __shared__ LogitsLds sh;
     extern __shared__ __attribute__((aligned(16))) uint32_t mask[];
-    auto logits = [&](size_t row) { return (const typename E::raw *)a.logits + row * a.stride; };
-    auto grads = [&](size_t row) { return (typename E::raw *)a.grad + row * a.C; };
-    // the next row that counts from `row` on; ignored ones are done on the way
-    auto live = [&](size_t row) {
-        for (; row < a.rows; row += gridDim.x) {
-            if (!a.weights || a.weights[row] != 0.0f) break;
+    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
+        typename E::raw *out = (typename E::raw *)a.grad + row * a.C;
+        const float weight = a.weights ? a.weights[row] : 1.0f;
+        if (weight == 0.0f) {                                // ignored: 0 whatever it holds
             ignored_out(a, row);
-            zero_classes<E, NT>(grads(row), a.C);
+            zero_classes<E, NT>(out, a.C);
+            continue;
         }
-        return row;
-    };
-    size_t row = live(blockIdx.x);
-    if (row >= a.rows) return;
-    Row reg;
-    ListEntries en;
-    if (threadIdx.x < WAVE) en.load_list(a, row);
-    Span<E> span(logits(row), a.C);
-    reg.load(logits(row), span);
-    while (true) {
-        const typename E::raw *x = logits(row);
-        typename E::raw *out = grads(row);
+        ListEntries en;
+        if (threadIdx.x < WAVE) en.load_list(a, row);
+        const Span<E> span(x, a.C);
+        Row reg;
+        reg.template load<true>(x, span);
         if (BUCKET) mask_listed<E, NT>(a, row, 0, span, mask);
         if (threadIdx.x < WAVE) en.load_logits<E>(a, x);
         Running run = running_start(a.c);
@@ -1292,21 +1288,11 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
         const float3 j = block_join<NT>(run, a.c, sh);
         const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
         const ListTerms t = list_terms(a, st, sh);
-        const float weight = a.weights ? a.weights[row] : 1.0f;
         if (threadIdx.x < WAVE) loss_out(a, row, weight, st, t, sh);
-
-        const size_t next = live(row + gridDim.x);
-        const bool more = next < a.rows;
-        const typename E::raw *nx = logits(more ? next : row);
-        const Span<E> nspan(nx, a.C);
-        const uint32_t fetch = more ? nspan.nvec : 0;
-        if (more && threadIdx.x < WAVE) en.load_list(a, next);
         const float coef = weight * a.t * a.scale, dense = coef * t.dense;
         const bool none = t.m == -INFINITY || st.m == -INFINITY;     // nothing has a probability, or nothing off the list
         auto value = [&](float v) { return none ? 0.0f : exp2_hw((v - st.m) * a.c - st.l2) * dense; };
         typename E::raw *to = out + span.head;
-        if (reg.tid < span.edges) out[span.edge(reg.tid)] = E::put(value(reg.edge));
-        reg.edge = more && reg.tid < nspan.edges ? E::get(nx[nspan.edge(reg.tid)]) : -INFINITY;
 #pragma unroll
         for (int k = 0; k < Row::R; ++k) {
             const uint32_t i = k * NT + reg.tid;
@@ -1315,17 +1301,12 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
                 E::unpack(reg.w[k], v);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[e] = value(v[e]);
-                store_raw<E>(to + (size_t)i * VEC, E::pack(v));
+                store_raw<E, NT == 1024>(to + (size_t)i * VEC, E::pack(v));
             }
-            reg.w[k] = E::none();
-            if (i < fetch) reg.w[k] = load_raw<E>(nx + nspan.head + (size_t)i * VEC);
         }
+        if (reg.tid < span.edges) out[span.edge(reg.tid)] = E::put(value(reg.edge));
         if (t.m != -INFINITY) listed_grad<E, NT>(a, coef, t, out, a.C, 0, sh);
         else __syncthreads();
-        if (!more) break;
-        row = next;
-        span = nspan;
-        reg.forget_thread();
     }
 }
 
@@ -1790,13 +1771,22 @@ static Split split_rows(size_t rows, uint32_t C, uint32_t blocks, uint32_t most)
     return {(C + seg - 1) / seg, seg};
 }
 constexpr uint32_t FILL_BLOCKS = 1024;
-static uint32_t fuse_rows() { const char *e = getenv("LG_FUSE"); return e ? atoi(e) : 512; }
+// Loss and gradient by whole rows from this many on: below, segments fill the chip better (rows of 50021 float32, both ways:
+// 300 rows 48 / 46 us, 520 rows 75 / 73, 777 rows 99 / 115; 520 rows of 9000 classes 30 / 33).
+constexpr size_t FUSE_ROWS = 512;
 // What a block of NT threads holds in registers.
 static uint32_t resident(int dtype, int nt) { return 16u * nt * (dtype == ODBOX_DTYPE_F32 ? 4 : 8); }
 static Split score_split(size_t rows, uint32_t C, int k, int dtype) { return split_rows(rows, C, FILL_BLOCKS, k ? resident(dtype, 1024) : 1u << 24); }
 static Split distill_split(size_t rows, uint32_t C)
 {
     return split_rows(rows, C, FILL_BLOCKS, MASK_CLASSES);
+}
+// Logits that nobody reads again (no statistics are kept for a gradient) and that the 256 MB Infinity Cache could not hold are read around
+// the caches: 2048 x 131072 bfloat16 scores 99 -> 92 us, 2048 x 32768 float32 losses 53 -> 49 us.  Ahead of a gradient the same loads cost
+// what its second read then misses (1021 x 100003 float16 both ways 126 -> 146 us).
+static bool passes(size_t rows, int C, int dtype, const void *stats)
+{
+    return !stats && rows * C > ((size_t)256 << 20) / (dtype == ODBOX_DTYPE_F32 ? 4 : 2);
 }
 // Blocks that stay: as many as the 256 CUs hold at four waves a SIMD (128 registers).
 static dim3 staying_grid(size_t work, int nt)
@@ -1896,7 +1886,8 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
             constexpr int NT = decltype(nt)::value;
             LOGITS_LAUNCH(dtype, (score_top_kernel<E, NT>), staying_grid(rows * sp.segs, NT), dim3(NT), 0, st, a);
         });
-    else LOGITS_LAUNCH(dtype, (score_kernel<E, 256>), grid, dim3(256), 0, st, a);
+    else if (passes(rows, C, dtype, out_stats)) LOGITS_LAUNCH(dtype, (score_kernel<E, 256, true>), grid, dim3(256), 0, st, a);
+    else LOGITS_LAUNCH(dtype, (score_kernel<E, 256, false>), grid, dim3(256), 0, st, a);
     if (sp.segs > 1) LOGITS_LAUNCH(dtype, score_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);
     return launch_status("label_logprobs");
 }
@@ -1989,7 +1980,7 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
     double *partial = (double *)workspace;
     float *per_row = out_rows ? out_rows : (float *)(partial + SUM_BLOCKS);
     const bool is_short = C <= short_limit(dtype);
-    const bool fused = grad && !is_short && rows >= fuse_rows() && (uint32_t)C <= resident(dtype, 1024);
+    const bool fused = grad && !is_short && rows >= FUSE_ROWS && (uint32_t)C <= resident(dtype, 1024);
     const Split sp = fused ? Split{1, (uint32_t)C} : distill_split(rows, (uint32_t)C);
     float4 *spare = (float4 *)((float *)(partial + SUM_BLOCKS) + (rows + 3) / 4 * 4);
     float4 *keep = out_stats ? (float4 *)out_stats : grad ? spare : nullptr;
@@ -2007,8 +1998,14 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
             else LOGITS_LAUNCH(dtype, (distill_fused_kernel<E, NT, false>), staying_grid(rows, NT), dim3(NT), 0, st, a);
         });
     } else {
-        if (rest == ODBOX_REST_BUCKET) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true>), grid, dim3(256), mask_bytes(256), st, a);
-        else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false>), grid, dim3(256), 0, st, a);
+        const bool passing = passes(rows, C, dtype, keep);
+        if (rest == ODBOX_REST_BUCKET) {
+            if (passing) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true, true>), grid, dim3(256), mask_bytes(256), st, a);
+            else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true, false>), grid, dim3(256), mask_bytes(256), st, a);
+        } else {
+            if (passing) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false, true>), grid, dim3(256), 0, st, a);
+            else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false, false>), grid, dim3(256), 0, st, a);
+        }
         if (sp.segs > 1) LOGITS_LAUNCH(dtype, distill_join_kernel<E>, work_grid(rows), dim3(WAVE), 0, st, a);
         if (grad) LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, 256>), grid, dim3(256), 0, st, a);
     }
