@@ -349,6 +349,78 @@ def test_teacher_to_student_step():
     assert torch.isfinite(step())
 
 
+def _sample(rows):
+    """A few rows of many: the first, the last and some between."""
+    return sorted({0, 1, rows // 3, rows // 2, rows - 2, rows - 1})
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('rows,C,k', [(1030, 1500, 33), (1100, 4100, 128), (1030, 9001, 5), (1100, 16390, 64), (1030, 40003, 20), (1030, 70001, 128)])
+def test_many_long_rows_with_top_classes(rows, C, k, dtype):
+    """Whole rows a block (few rows are split instead): some against the definition, all classes against the split kernel's."""
+    x = _make(C, rows, C, dtype)
+    labels = torch.arange(rows) % C
+    labels[3::7] = -1
+    r = M.label_logprobs(x, labels.cuda(), top_k=k)
+    at = _sample(rows)
+    check_scores(x[at], labels[at], k, 1.0, M.LabelLogprobs(r.logprobs[at], r.entropy[at], r.top_logprobs[at], r.top_labels[at]))
+    few = M.label_logprobs(x[:200], labels[:200].cuda(), top_k=k)
+    assert torch.equal(r.top_labels[:200], few.top_labels)
+
+
+@pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('rows,C,K,pad', [(530, 2100, 128, 0), (600, 3001, 7, 5), (520, 9000, 33, 0), (530, 16001, 64, 2), (520, 33333, 5, 0),
+                                          (515, 65537, 20, 0), (515, 131073, 9, 0)])
+def test_many_long_rows_with_their_gradient(rows, C, K, pad, dtype, rest):
+    """The one-read kernel and, where a row does not fit a block's registers, the kernels beside it; masked rows among them."""
+    x = _make(C, rows, C, dtype, pad=pad)
+    tl, ids = _list(C, x, K, 1.0)
+    w = torch.rand(rows, generator=torch.Generator().manual_seed(5)).cuda() + 0.5
+    w[1::5] = 0.0
+    x[rows // 2] = -INF
+    x[rows // 3, : C // 2] = torch.finfo(dtype).min
+    ids[rows - 1, 1:3] = ids[rows - 1, 0]
+    ids[0, -1] = -1
+    losses, grad = M.distill_loss(x, tl, ids, rest=rest, row_weights=w, reduction=None, return_grad=True)
+    at = _sample(rows)
+    check_distill(x[at], tl[at], ids[at], 1.0, rest, w[at], losses[at], grad[at])
+    assert (losses[1::5] == 0).all() and (grad[1::5] == 0).all() and losses[rows // 2].item() == 0 and (grad[rows // 2] == 0).all()
+    xg = x.detach().requires_grad_()
+    l2 = M.distill_loss(xg, tl, ids, rest=rest, row_weights=w, reduction=None)
+    g2, = torch.autograd.grad(l2.sum(), xg)
+    check_distill(x[at], tl[at], ids[at], 1.0, rest, w[at], l2[at], g2[at])
+    # Every row both ways.  A probability is off by at most u (4 |t| + 4 + adds + 4 l2) relative, |t| < 120 and l2 < 17 here, and a
+    # gradient by half a step of its type.  Off a renormalised list the gradient is a product with p; elsewhere it is a
+    # difference of probabilities (at most w), so that the same error counts absolutely.
+    rel = 2 * R.U * (4 * 120 + 4 + R.adds(C) + 4 * 17)
+    a, b = grad.double(), g2.double()
+    differences = torch.zeros_like(a)
+    if rest == 'bucket':
+        differences += w[:, None]
+    else:
+        differences.scatter_(1, ids.clamp(min=0).long(), w.double()[:, None].expand(-1, K).contiguous())
+    assert ((a - b).abs() <= (2 * R.EPS[dtype] + rel) * a.abs() + rel * differences + 2 * R.TINY[dtype]).all()
+
+
+@pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
+def test_more_logits_than_the_caches_hold(rest):
+    rows, C = 1100, 131075                                       # 288 MB, rows at odd addresses
+    x = _make(1, 11, C, BF16)[torch.arange(rows).cuda() % 11]
+    labels = (torch.arange(rows) * 119) % C
+    at = _sample(rows)
+    r = M.label_logprobs(x, labels.cuda())
+    check_scores(x[at], labels[at], 0, 1.0, M.LabelLogprobs(r.logprobs[at], r.entropy[at], None, None))
+    tl, ids = _list(2, x[:11], 16, 1.0)
+    pick = torch.arange(rows).cuda() % 11
+    losses = M.distill_loss(x, tl[pick], ids[pick], rest=rest, reduction=None)
+    check_distill(x[at], tl[pick][at], ids[pick][at], 1.0, rest, None, losses[at])
+    assert torch.equal(losses[:88], losses[88:176])              # the same rows on the same boundaries (8 rows of 131075 apart)
+    xg = x.detach().requires_grad_()
+    g, = torch.autograd.grad(M.label_logprobs(xg, labels.cuda()).logprobs.sum(), xg)
+    check_score_grad(x[at], labels[at], 0, 1.0, np.ones(len(at)), np.zeros(len(at)), np.zeros((len(at), 1)), [[0]] * len(at), g[at])
+
+
 def test_results_do_not_change_from_call_to_call():
     x = _make(1, 40, 30011, BF16)
     x = (x.float() * 4).round().div(4).to(BF16)                 # many ties
