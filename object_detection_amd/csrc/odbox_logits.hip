@@ -51,6 +51,16 @@ struct F16 {
     static constexpr int VEC = 8;
     static __device__ __forceinline__ float get(raw v) { return (float)v; }
     static __device__ __forceinline__ raw put(float v) { return (_Float16)v; }
+    // the 16 bits of a value as an unsigned number of the same order (-0 folded into +0, NaN above all), and back
+    static __device__ __forceinline__ uint32_t order16(float v)
+    {
+        const uint32_t u = __builtin_bit_cast(uint16_t, (_Float16)(v + 0.0f));
+        return v != v ? 0xffffu : u & 0x8000u ? u ^ 0xffffu : u | 0x8000u;
+    }
+    static __device__ __forceinline__ float value16(uint32_t o)
+    {
+        return o == 0xffffu ? NAN : (float)__builtin_bit_cast(_Float16, (uint16_t)(o & 0x8000u ? o & 0x7fffu : o ^ 0xffffu));
+    }
     static __device__ __forceinline__ void unpack(u32x4 w, float *v)
     {
         const f16x8 h = __builtin_bit_cast(f16x8, w);
@@ -71,6 +81,11 @@ struct BF16 {
     static constexpr int VEC = 8;
     static __device__ __forceinline__ float get(raw v) { return __uint_as_float((uint32_t)v << 16); }
     static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(raw, (__bf16)v); }
+    static __device__ __forceinline__ uint32_t order16(float v) { return v != v ? 0xffffu : f32_ordered(v) >> 16; }
+    static __device__ __forceinline__ float value16(uint32_t o)
+    {
+        return o == 0xffffu ? NAN : __uint_as_float((o & 0x8000u ? o & 0x7fffu : o ^ 0xffffu) << 16);
+    }
     static __device__ __forceinline__ void unpack(u32x4 w, float *v)
     {
 #pragma unroll
@@ -577,18 +592,21 @@ __device__ __forceinline__ void top_classes(Resident<E, NT> &r, const typename E
                 top.group[part * 64 + threadIdx.x] = f32_ordered(vmax(part == 0 ? g[0] : part == 1 ? g[1] : part == 2 ? g[2] : g[3], M_START));
         }
         const float tau = f32_unordered(top_threshold<NT>(G, k, sh, top));
-        // candidates by wave: a ballot per value, so positions need no atomics and their order no luck
+        // Candidates by wave: a ballot per value, so positions need no atomics and their order no luck.  A miss costs two
+        // instructions; what a hit stores (value and index, made a key later) is kept short, some 22 of a wave's 8192 values hit.
+        const uint32_t mine = span.head + r.tid * VEC;
+        uint2 *list = (uint2 *)top.key + wave * ROOM;
         auto look = [&](float v, uint32_t at) {
             const uint64_t hit = __ballot(v >= tau);
             if (hit == 0) return;
             const uint32_t pos = have + __builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0u));
-            if (v >= tau && pos < ROOM) top.key[wave * ROOM + pos] = top_key(v, first + at);
+            if (v >= tau && pos < ROOM) list[pos] = make_uint2(__float_as_uint(v), at);
             have += __popcll(hit);
         };
         if (__any(m >= tau)) {
             r.each(span, [&](int kk, const float *v) {
 #pragma unroll
-                for (int j = 0; j < Resident<E, NT>::N; ++j) look(v[j], span.head + ((kk + j / VEC) * NT + r.tid) * VEC + j % VEC);
+                for (int j = 0; j < Row::N; ++j) look(v[j], mine + (kk + j / VEC) * NT * VEC + j % VEC);
             });
             look(r.edge, span.edge(r.tid));
         }
@@ -597,11 +615,26 @@ __device__ __forceinline__ void top_classes(Resident<E, NT> &r, const typename E
     if (ok) {
         // the waves' lists side by side (places beyond the span hold -inf, tau is M_START or more: they never count)
         const bool over = have > ROOM;
-        if (WAVES > 1) {
-            uint64_t mine[(ROOM + 63) / 64];
+        const uint2 *list = (const uint2 *)top.key + wave * ROOM;
+        uint64_t key[(ROOM + 63) / 64 < 4 ? (ROOM + 63) / 64 : 4];       // (a single wave's list may be longer: in place, piece by piece)
+        constexpr uint32_t PIECE = sizeof(key) / 8 * 64;
+        auto read = [&](uint32_t from) {
 #pragma unroll
-            for (uint32_t i = 0; i < (ROOM + 63) / 64; ++i)
-                if (i * 64 + lane < have && !over) mine[i] = top.key[wave * ROOM + i * 64 + lane];
+            for (uint32_t i = 0; i < PIECE / 64; ++i) {
+                const uint32_t t = from + i * 64 + lane;
+                if (t < have) key[i] = top_key(__uint_as_float(list[t].x), first + list[t].y);
+            }
+        };
+        auto write = [&](uint32_t from, uint32_t to) {
+#pragma unroll
+            for (uint32_t i = 0; i < PIECE / 64; ++i) {
+                const uint32_t t = i * 64 + lane;
+                if (from + t < have) top.key[to + t] = key[i];
+            }
+        };
+        if (WAVES > 1) {
+            static_assert(WAVES == 1 || PIECE >= ROOM, "a wave's list fits one piece");
+            if (!over) read(0);
             if (lane == 0) sh.f[wave] = over ? 1e9f : (float)have;
             __syncthreads();
             uint32_t base = 0, all = 0;
@@ -611,13 +644,13 @@ __device__ __forceinline__ void top_classes(Resident<E, NT> &r, const typename E
                 all += c;
             }
             few = all >= k && all <= TOP_CAP;
-            if (few)
-#pragma unroll
-                for (uint32_t i = 0; i < (ROOM + 63) / 64; ++i)
-                    if (i * 64 + lane < have) top.key[base + i * 64 + lane] = mine[i];
+            if (few) write(0, base);
             have = all;
-        } else
+        } else {
             few = have >= k && !over;
+            if (few)
+                for (uint32_t from = 0; from < have; from += PIECE) read(from), write(from, from);
+        }
         __syncthreads();
         if (few) rank_candidates<NT>(have, k, top, out);
         __syncthreads();
@@ -1349,7 +1382,8 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(DistillArgs a)
 // lane exchanges, and no barrier is needed.  S is the exact number of steps, so only the last one looks at the row's end.  The last vector of a row that is no multiple of a vector is read (and
 // written) back from the row's end, its first values counting as dropped: no access leaves the row.
 constexpr int SHORT_THREADS = 256;
-constexpr int SHORT_STEPS = 4;
+template <class E>
+constexpr int SHORT_STEPS = E::VEC == 4 ? 6 : 4;              // 24 or 32 values a lane
 
 template <int L>
 __device__ __forceinline__ float group_max(float x)
@@ -1358,7 +1392,7 @@ __device__ __forceinline__ float group_max(float x)
     x = vmax(x, dpp_f<0x4E, 0xf>(x, x));                     // quad_perm [2,3,0,1]
     if (L >= 8) x = vmax(x, dpp_f<0x141, 0xf>(x, x));       // row_half_mirror
     if (L >= 16) x = vmax(x, dpp_f<0x140, 0xf>(x, x));       // row_mirror
-    if (L >= 64) x = vmax(x, __shfl_xor(x, 16));
+    if (L >= 32) x = vmax(x, __shfl_xor(x, 16));
     if (L >= 64) x = vmax(x, __shfl_xor(x, 32));
     return x;
 }
@@ -1369,7 +1403,7 @@ __device__ __forceinline__ float group_sum(float x)
     x += dpp_f<0x4E, 0xf>(x, x);
     if (L >= 8) x += dpp_f<0x141, 0xf>(x, x);
     if (L >= 16) x += dpp_f<0x140, 0xf>(x, x);
-    if (L >= 64) x += __shfl_xor(x, 16);
+    if (L >= 32) x += __shfl_xor(x, 16);
     if (L >= 64) x += __shfl_xor(x, 32);
     return x;
 }
@@ -1382,7 +1416,7 @@ __device__ __forceinline__ uint32_t group_fold(uint32_t x, Op op)
     x = op(x, dpp_u<0x4E>(x));
     if (L >= 8) x = op(x, dpp_u<0x141>(x));
     if (L >= 16) x = op(x, dpp_u<0x140>(x));
-    if (L >= 64) x = op(x, (uint32_t)__shfl_xor(x, 16));
+    if (L >= 32) x = op(x, (uint32_t)__shfl_xor(x, 16));
     if (L >= 64) x = op(x, (uint32_t)__shfl_xor(x, 32));
     return x;
 }
@@ -1395,7 +1429,10 @@ struct ShortRow {
     float v[PV];
     uint32_t lane, C;
 
-    __device__ __forceinline__ ShortRow(uint32_t classes) : lane(threadIdx.x % L), C(classes) {}
+    __device__ __forceinline__ ShortRow(uint32_t classes) : lane(threadIdx.x % L), C(classes)
+    {
+        asm volatile("" : "+v"(lane));                       // what is computed from it is not kept from row to row
+    }
     __device__ __forceinline__ bool tiny() const { return TINY && C < VEC; }
     __device__ __forceinline__ uint32_t base(int k) const
     {
@@ -1494,26 +1531,42 @@ __global__ __launch_bounds__(SHORT_THREADS) void score_short_kernel(ScoreArgs a)
             if (a.stats) a.stats[row] = make_float4(st.m, st.l2, st.ent, 0.0f);
         }
         if (a.k == 0) continue;
-        // one round a class: the largest value left, the lowest class that has it; 0 stands for a value that is gone
+        // One round a class: the largest value left, the lowest class that has it; 0 stands for a value that is gone.  A 16-bit value
+        // and its class make one number, so that there the maximum names the class and no two are equal.
+        constexpr bool PAIR = Row::VEC == 8;
         uint32_t o[Row::PV];
 #pragma unroll
-        for (int i = 0; i < Row::PV; ++i) o[i] = !r.counts(i / Row::VEC, i % Row::VEC) ? 0u : r.v[i] != r.v[i] ? 0xffffffffu : f32_ordered(r.v[i]);
+        for (int i = 0; i < Row::PV; ++i) {
+            const int k = i / Row::VEC, e = i % Row::VEC;
+            const float v = r.v[i];
+            if constexpr (PAIR) o[i] = (E::order16(v) << 16) | (0xffffu - (r.base(k) + e));
+            else o[i] = v != v ? 0xffffffffu : f32_ordered(v);
+            if (!r.counts(k, e)) o[i] = 0;
+        }
         float keep_lp = 0.0f;
         int32_t keep_id = 0;
         for (uint32_t round = 0; round < a.k; ++round) {
-            uint32_t best = 0;
+            uint32_t best = 0, win = 0xffffffffu;
 #pragma unroll
             for (int i = 0; i < Row::PV; ++i) best = o[i] > best ? o[i] : best;
             best = group_fold<L>(best, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
-            uint32_t win = 0xffffffffu;
+            float v;
+            if constexpr (PAIR) {
+                win = 0xffffu - (best & 0xffffu);
+                v = E::value16(best >> 16);
 #pragma unroll
-            for (int i = Row::PV - 1; i >= 0; --i) win = o[i] == best ? r.base(i / Row::VEC) + i % Row::VEC : win;
-            win = group_fold<L>(win, [](uint32_t p, uint32_t q) { return p < q ? p : q; });
+                for (int i = 0; i < Row::PV; ++i) o[i] = o[i] == best ? 0u : o[i];
+            } else {
 #pragma unroll
-            for (int i = 0; i < Row::PV; ++i) o[i] = win - r.base(i / Row::VEC) == (uint32_t)(i % Row::VEC) ? 0u : o[i];
+                for (int i = Row::PV - 1; i >= 0; --i) win = o[i] == best ? r.base(i / Row::VEC) + i % Row::VEC : win;
+                win = group_fold<L>(win, [](uint32_t p, uint32_t q) { return p < q ? p : q; });
+#pragma unroll
+                for (int i = 0; i < Row::PV; ++i) o[i] = win - r.base(i / Row::VEC) == (uint32_t)(i % Row::VEC) ? 0u : o[i];
+                v = best == 0xffffffffu ? NAN : f32_unordered(best);
+            }
             if (round % L == r.lane) {
                 keep_id = (int32_t)win;
-                keep_lp = logprob_of<E>(a, st, best == 0xffffffffu ? NAN : f32_unordered(best));
+                keep_lp = logprob_of<E>(a, st, v);
             }
             if (round % L == L - 1 || round == a.k - 1) {    // L results at a time, side by side
                 const uint32_t at = round - round % L + r.lane;
@@ -1810,35 +1863,42 @@ static void resident_variant(int dtype, uint32_t n, F f)
         else { using E = BF16; hipLaunchKernelGGL(K_, __VA_ARGS__); }                        \
     } while (0)
 
-// A short row of nv vectors goes to the smallest group of 4, 8, 16 or 64 lanes that holds it in SHORT_STEPS steps.
-static int short_limit(int dtype) { return 64 * SHORT_STEPS * (dtype == ODBOX_DTYPE_F32 ? 4 : 8); }
+// A short row of nv vectors goes to the smallest group of 4, 8, .. 64 lanes that holds it in SHORT_STEPS steps.
+static int short_limit(int dtype) { return dtype == ODBOX_DTYPE_F32 ? 64 * SHORT_STEPS<F32> * 4 : 64 * SHORT_STEPS<F16> * 8; }
 static dim3 short_grid(size_t rows, int L)
 {
     const size_t per = SHORT_THREADS / L;
     return work_grid((rows + per - 1) / per);
 }
+template <int V>
+using Constant = std::integral_constant<int, V>;
+template <class E, int L, int S, class F>
+static void short_lanes(int nv, F f)
+{
+    if (nv > L * SHORT_STEPS<E>) {
+        if constexpr (L < 64) short_lanes<E, 2 * L, SHORT_STEPS<E> / 2 + 1>(nv, f);
+    } else if (nv > L * S) {
+        if constexpr (S < SHORT_STEPS<E>) short_lanes<E, L, S + 1>(nv, f);
+    } else
+        f(E(), Constant<L>(), Constant<S>());
+}
 template <class F>
 static void short_variant(int dtype, int C, F f)
 {
-    const int vec = dtype == ODBOX_DTYPE_F32 ? 4 : 8, nv = (C + vec - 1) / vec;
-    auto steps = [&](auto lanes, auto s) { f(lanes, s); };
-    using std::integral_constant;
-#define ODBOX_SHORT(L_, S_) steps(integral_constant<int, L_>(), integral_constant<int, S_>())
-    if (nv <= 4) ODBOX_SHORT(4, 1);
-    else if (nv <= 8) ODBOX_SHORT(4, 2);
-    else if (nv <= 12) ODBOX_SHORT(4, 3);
-    else if (nv <= 16) ODBOX_SHORT(4, 4);
-    else if (nv <= 24) ODBOX_SHORT(8, 3);
-    else if (nv <= 32) ODBOX_SHORT(8, 4);
-    else if (nv <= 48) ODBOX_SHORT(16, 3);
-    else if (nv <= 64) ODBOX_SHORT(16, 4);
-    else if (nv <= 128) ODBOX_SHORT(64, 2);
-    else if (nv <= 192) ODBOX_SHORT(64, 3);
-    else ODBOX_SHORT(64, 4);
-#undef ODBOX_SHORT
+    if (dtype == ODBOX_DTYPE_F32) short_lanes<F32, 4, 1>((C + 3) / 4, f);
+    else if (dtype == ODBOX_DTYPE_F16) short_lanes<F16, 4, 1>((C + 7) / 8, f);
+    else short_lanes<BF16, 4, 1>((C + 7) / 8, f);
 }
-// The rounds of the short kernel's selection against the block's threshold.
-static bool score_is_short(int dtype, int C, int k) { return C <= short_limit(dtype) && (k <= 16 || C <= 128); }
+// The short kernel's selection costs a round for every class on L lanes, the wave's threshold about the same for any k.  Measured
+// (float32, rounds / threshold): 100 000 x 300, k 32 (16 lanes) 162 / 281 us; 40 000 x 600, k 16 (32 lanes) 77 / 97;
+// 20 000 x 1000, k 10 (64 lanes) 49 / 55; 20 000 x 1400, k 20 (64 lanes) 110 / 62.
+static bool score_is_short(int dtype, int C, int k)
+{
+    if (C > short_limit(dtype)) return false;
+    int lanes = 64;
+    short_variant(dtype, C, [&](auto, auto l, auto) { lanes = decltype(l)::value; });
+    return lanes == 4 || k * lanes <= 640;
+}
 
 }  // namespace odbox
 
@@ -1875,9 +1935,10 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid = work_grid(rows * sp.segs);
     if (score_is_short(dtype, C, top_k)) {
-        short_variant(dtype, C, [&](auto l, auto n) {
+        short_variant(dtype, C, [&](auto e, auto l, auto n) {
+            using E = decltype(e);
             constexpr int L = decltype(l)::value, S = decltype(n)::value;
-            LOGITS_LAUNCH(dtype, (score_short_kernel<E, L, S>), short_grid(rows, L), dim3(SHORT_THREADS), 0, st, a);
+            hipLaunchKernelGGL((score_short_kernel<E, L, S>), short_grid(rows, L), dim3(SHORT_THREADS), 0, st, a);
         });
         return launch_status(name);
     }
@@ -1910,9 +1971,10 @@ int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, in
                        labels, top_labels, (const float4 *)stats, upstream_logprobs, upstream_entropy, upstream_top, grad, sp.segs, sp.seg};
     const dim3 grid = work_grid(rows * sp.segs);
     if (C <= short_limit(dtype)) {
-        short_variant(dtype, C, [&](auto l, auto n) {
+        short_variant(dtype, C, [&](auto e, auto l, auto n) {
+            using E = decltype(e);
             constexpr int L = decltype(l)::value, S = decltype(n)::value;
-            LOGITS_LAUNCH(dtype, (score_grad_short_kernel<E, L, S>), short_grid(rows, L), dim3(SHORT_THREADS), 0, (hipStream_t)stream, a);
+            hipLaunchKernelGGL((score_grad_short_kernel<E, L, S>), short_grid(rows, L), dim3(SHORT_THREADS), 0, (hipStream_t)stream, a);
         });
         return launch_status(name);
     }
@@ -1935,16 +1997,17 @@ static int distill_check(const char *name, const void *logits, int dtype, size_t
 static void distill_short(int dtype, int rest, bool grad, const DistillArgs &a, hipStream_t st)
 {
     const size_t rows = a.rows;
-    short_variant(dtype, (int)a.C, [&](auto l, auto n) {
+    short_variant(dtype, (int)a.C, [&](auto e, auto l, auto n) {
+        using E = decltype(e);
         constexpr int L = decltype(l)::value, S = decltype(n)::value;
         const size_t lds = (size_t)(SHORT_THREADS / L) * ((a.C + 3) & ~3u) * sizeof(float);
         const dim3 grid = short_grid(rows, L), block(SHORT_THREADS);
         if (rest == ODBOX_REST_BUCKET) {
-            if (grad) LOGITS_LAUNCH(dtype, (distill_short_kernel<E, L, S, true, true>), grid, block, lds, st, a);
-            else LOGITS_LAUNCH(dtype, (distill_short_kernel<E, L, S, true, false>), grid, block, lds, st, a);
+            if (grad) hipLaunchKernelGGL((distill_short_kernel<E, L, S, true, true>), grid, block, lds, st, a);
+            else hipLaunchKernelGGL((distill_short_kernel<E, L, S, true, false>), grid, block, lds, st, a);
         } else {
-            if (grad) LOGITS_LAUNCH(dtype, (distill_short_kernel<E, L, S, false, true>), grid, block, lds, st, a);
-            else LOGITS_LAUNCH(dtype, (distill_short_kernel<E, L, S, false, false>), grid, block, 0, st, a);
+            if (grad) hipLaunchKernelGGL((distill_short_kernel<E, L, S, false, true>), grid, block, lds, st, a);
+            else hipLaunchKernelGGL((distill_short_kernel<E, L, S, false, false>), grid, block, 0, st, a);
         }
     });
 }
