@@ -1829,7 +1829,9 @@ constexpr uint32_t FILL_BLOCKS = 1024;
 constexpr size_t FUSE_ROWS = 512;
 // What a block of NT threads holds in registers.
 static uint32_t resident(int dtype, int nt) { return 16u * nt * (dtype == ODBOX_DTYPE_F32 ? 4 : 8); }
-static Split score_split(size_t rows, uint32_t C, int k, int dtype) { return split_rows(rows, C, FILL_BLOCKS, k ? resident(dtype, 1024) : 1u << 24); }
+// With top classes a segment fits 256 threads' registers, however many rows there are: blocks of 1024 threads wait longer at their
+// barriers than the join takes (2048 x 131072 bfloat16, 20 classes 155 / 191 us; 4096 x 50000, 8 classes 133 / 206 us).
+static Split score_split(size_t rows, uint32_t C, int k, int dtype) { return split_rows(rows, C, FILL_BLOCKS, k ? resident(dtype, 256) : 1u << 24); }
 static Split distill_split(size_t rows, uint32_t C)
 {
     return split_rows(rows, C, FILL_BLOCKS, MASK_CLASSES);
@@ -1942,11 +1944,8 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
         });
         return launch_status(name);
     }
-    if (top_k)
-        resident_variant(dtype, sp.seg, [&](auto nt) {
-            constexpr int NT = decltype(nt)::value;
-            LOGITS_LAUNCH(dtype, (score_top_kernel<E, NT>), staying_grid(rows * sp.segs, NT), dim3(NT), 0, st, a);
-        });
+    if (top_k && sp.seg <= resident(dtype, 64)) LOGITS_LAUNCH(dtype, (score_top_kernel<E, 64>), staying_grid(rows * sp.segs, 64), dim3(64), 0, st, a);
+    else if (top_k) LOGITS_LAUNCH(dtype, (score_top_kernel<E, 256>), staying_grid(rows * sp.segs, 256), dim3(256), 0, st, a);
     else if (passes(rows, C, dtype, out_stats)) LOGITS_LAUNCH(dtype, (score_kernel<E, 256, true>), grid, dim3(256), 0, st, a);
     else LOGITS_LAUNCH(dtype, (score_kernel<E, 256, false>), grid, dim3(256), 0, st, a);
     if (sp.segs > 1) LOGITS_LAUNCH(dtype, score_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);

@@ -403,6 +403,20 @@ def test_many_long_rows_with_their_gradient(rows, C, K, pad, dtype, rest):
     assert ((a - b).abs() <= (2 * R.EPS[dtype] + rel) * a.abs() + rel * differences + 2 * R.TINY[dtype]).all()
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_millions_of_classes(dtype):
+    rows, C = 2, 3000001
+    x = _make(7, rows, C, dtype)
+    labels = torch.tensor([C - 1, 5])
+    r = M.label_logprobs(x, labels.cuda(), top_k=128)
+    check_scores(x, labels, 128, 1.0, r)
+    tl, ids = r.top_logprobs - 0.5, r.top_labels.clone()
+    ids[1, 3] = C - 1
+    for rest in ('renormalise', 'bucket'):
+        losses, grad = M.distill_loss(x, tl, ids, rest=rest, reduction=None, return_grad=True)
+        check_distill(x, tl, ids, 1.0, rest, None, losses, grad)
+
+
 @pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
 def test_more_logits_than_the_caches_hold(rest):
     rows, C = 1100, 131075                                       # 288 MB, rows at odd addresses
