@@ -305,7 +305,8 @@ int odbox_decode_nms_mixed(const float *anchors /*[N,4] or NULL*/, const void *r
 /* logits: [rows, C] of `dtype` (ODBOX_DTYPE_*), the classes of a row side by side, rows row_stride ELEMENTS apart (>= C, or 0
  * for one row read again and again); aligned to their element only.  Every result is computed in fp32 from the widened values.
  * A logit of -inf is a class without probability.  A row whose logits are ALL -inf is empty: log-probabilities -inf, entropy 0,
- * losses and gradients 0.  A row that holds a NaN or +inf gives NaN. */
+ * losses and gradients 0.  A row that holds a NaN or +inf gives NaN.  A row's sums are added in an order that depends on its length,
+ * the number of rows and where it starts modulo 16 bytes; the same call gives the same bits.  No output may overlap an input. */
 #define ODBOX_MAX_LOGITS 16777216   /* C: a class id is 24 bits of the selection key */
 #define ODBOX_MAX_TOP    128        /* top alternatives of a row, classes of a teacher's list */
 

@@ -1051,6 +1051,7 @@ __device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEnt
 #pragma unroll
     for (int h = 0; h < 2; ++h) sh.id[lane + 64 * h] = en.id[h];
     if (lane < 3) sh.id[128 + lane] = -1;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (one wave's LDS accesses stay in order)
     float mass, q0 = 0.0f;
     if (!a.bucket) {
         const float tm = wave_max(vmax(en.t[0], en.t[1]));
@@ -1798,7 +1799,7 @@ static int logits_check(const char *name, const void *logits, int dtype, size_t 
     if (dtype != ODBOX_DTYPE_F32 && dtype != ODBOX_DTYPE_F16 && dtype != ODBOX_DTYPE_BF16)
         return fail(ODBOX_EINVAL, "%s: dtype %d is none of ODBOX_DTYPE_*", name, dtype);
     if (C < 1 || C > ODBOX_MAX_LOGITS) return fail(ODBOX_EINVAL, "%s: C = %d is not in 1..%d", name, C, ODBOX_MAX_LOGITS);
-    if (rows > (size_t)1 << 40 || stride > (size_t)1 << 40) return fail(ODBOX_EINVAL, "%s: rows or row_stride over 2^40", name);
+    if (rows > (size_t)1 << 32 || stride > (size_t)1 << 40) return fail(ODBOX_EINVAL, "%s: rows over 2^32 or row_stride over 2^40", name);
     if (!(temperature >= 1e-6f && temperature <= 1e6f)) return fail(ODBOX_EINVAL, "%s: temperature %g is not in 1e-6..1e6", name, (double)temperature);
     if (rows && !logits) return fail(ODBOX_EINVAL, "%s: NULL logits", name);
     if ((uintptr_t)logits % (dtype == ODBOX_DTYPE_F32 ? 4 : 2)) return fail(ODBOX_EINVAL, "%s: logits are not aligned to their element", name);
@@ -2045,7 +2046,7 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
     const bool fused = grad && !is_short && rows >= FUSE_ROWS && (uint32_t)C <= resident(dtype, 1024);
     const Split sp = fused ? Split{1, (uint32_t)C} : distill_split(rows, (uint32_t)C);
     float4 *spare = (float4 *)((float *)(partial + SUM_BLOCKS) + (rows + 3) / 4 * 4);
-    float4 *keep = out_stats ? (float4 *)out_stats : grad ? spare : nullptr;
+    float4 *keep = out_stats ? (float4 *)out_stats : grad && !is_short && !fused ? spare : nullptr;
     DistillArgs a = {logits, rows, row_stride, (uint32_t)C, (uint32_t)K, LOG2E / temperature, temperature, 1.0f / temperature, scale, rest,
                      teacher_logprobs, teacher_labels, row_weights, per_row, keep, nullptr, 0, grad, sp.segs, sp.seg, spare + rows};
     const dim3 grid = work_grid(rows * sp.segs);

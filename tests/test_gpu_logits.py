@@ -600,6 +600,33 @@ def test_gradient_of_a_broadcast_row():
     torch.testing.assert_close(g, torch.stack(each).sum(0), rtol=0, atol=16 * R.U)
 
 
+@pytest.mark.parametrize('C', [90, 5000])
+def test_gradients_without_labels_and_of_some_outputs(C):
+    x = _make(C, 6, C, F32).requires_grad_()
+    r = M.label_logprobs(x, top_k=2)
+    assert r.logprobs is None and r.entropy.requires_grad and r.top_logprobs.requires_grad and not r.top_labels.requires_grad
+    g, = torch.autograd.grad(r.top_logprobs[:, 1].sum(), x, retain_graph=True)
+    up = np.zeros((6, 2))
+    up[:, 1] = 1
+    check_score_grad(x, torch.full((6,), -1), 2, 1.0, np.zeros(6), np.zeros(6), up, r.top_labels.tolist(), g)
+    g2, = torch.autograd.grad(r.top_logprobs[:, 1].sum(), x)     # the same graph once more
+    assert torch.equal(g, g2)
+    with torch.no_grad():
+        assert not M.label_logprobs(x).entropy.requires_grad
+    y = torch.randn(3, C, device='cuda', dtype=torch.float64, requires_grad=True)
+    g, = torch.autograd.grad(M.label_logprobs(y, torch.zeros(3, dtype=torch.int64)).logprobs.sum(), y)
+    assert g.dtype == torch.float64 and g.shape == y.shape
+
+
+def test_inputs_changed_before_the_backward_pass_are_noticed():
+    x = _make(1, 4, 50, F32).requires_grad_()
+    tl, ids = _list(1, x.detach(), 3, 1.0)
+    loss = M.distill_loss(x, tl, ids)
+    ids.zero_()
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
 def test_python_refusals():
     x = torch.zeros(4, 10, device='cuda')
     ids = torch.zeros(4, 3, dtype=torch.int32)
