@@ -4,6 +4,7 @@
 
 hipcc cross-compiles without a GPU.  -ffp-contract=off is part of the numerical contract
 (no FMA contraction: the reference rounds every fp32 op separately)."""
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -114,15 +115,19 @@ def build(force=False, verbose=False):
     hipcc = os.environ.get('HIPCC', 'hipcc')
     hooks = [f for f in tuning_flags() if not f.startswith('@train:')]
     os.makedirs(OBJ, exist_ok=True)
-    objs = []
-    for unit, extra in UNITS.items():
+
+    def compile_unit(unit):
         obj = os.path.join(OBJ, unit.replace('.hip', '.o'))
-        cmd = [hipcc] + COMMON + extra + hooks + ['-c', os.path.join(CSRC, unit), '-o', obj]
+        cmd = [hipcc] + COMMON + UNITS[unit] + hooks + ['-c', os.path.join(CSRC, unit), '-o', obj]
         if verbose:
             print(' '.join(cmd))
         subprocess.run(cmd, check=True)
-        objs.append(obj)
-    check_m0(hipcc, hooks, verbose)
+        return obj
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(UNITS) + 1) as pool:     # the units and the check's assembly
+        checked = pool.submit(check_m0, hipcc, hooks, verbose)
+        objs = list(pool.map(compile_unit, UNITS))
+        checked.result()
     check_tail_vgprs()
     cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', OUT] + objs
     if verbose:
