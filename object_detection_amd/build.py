@@ -29,8 +29,9 @@ UNITS = {
     'odbox_infer.hip': ['-fno-honor-nans'],
     'odbox_eval.hip': [],
     'odbox_logits.hip': [],
+    'odbox_logits_short.hip': [],
 }
-HEADERS = [os.path.join(CSRC, 'odbox_common.h'), os.path.join(ROOT, 'include', 'odbox.h')]
+HEADERS = [os.path.join(CSRC, 'odbox_common.h'), os.path.join(CSRC, 'odbox_logits.h'), os.path.join(ROOT, 'include', 'odbox.h')]
 
 
 STAMP = os.path.join(OBJ, 'flags.txt')

@@ -8,146 +8,9 @@
 // far as float32 reaches.  Sums, maxima and outputs other than gradients are 32-bit floats.
 #include <type_traits>
 
-#include "odbox_common.h"
+#include "odbox_logits.h"
 
 namespace odbox {
-
-constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float LN2 = 0.69314718055994530942f;
-constexpr float T_FLOOR = -16384.0f;             // stands for log2 p = -inf in p * log2 p (2^-16384 is 0, so the product is 0)
-constexpr float M_START = -1e30f;                // a running maximum before any class; times c it is still finite
-
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-// Element types: 16-byte vectors that may start at any element (rows of an odd number of classes do: global_load / store_dwordx4
-// take any alignment).  Stores round to nearest even.
-template <class V, int ALIGN>
-struct Unaligned {
-    typedef V type __attribute__((aligned(ALIGN)));
-};
-struct F32 {
-    using raw = float;
-    static __device__ __forceinline__ u32x4 none() { return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}; }   // -inf
-    static constexpr int VEC = 4;
-    static __device__ __forceinline__ float get(raw v) { return v; }
-    static __device__ __forceinline__ raw put(float v) { return v; }
-    static __device__ __forceinline__ void unpack(u32x4 w, float *v)
-    {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
-    }
-    static __device__ __forceinline__ u32x4 pack(const float *v)
-    {
-        return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-    }
-};
-struct F16 {
-    using raw = _Float16;
-    static __device__ __forceinline__ u32x4 none() { return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u}; }
-    static constexpr int VEC = 8;
-    static __device__ __forceinline__ float get(raw v) { return (float)v; }
-    static __device__ __forceinline__ raw put(float v) { return (_Float16)v; }
-    // the 16 bits of a value as an unsigned number of the same order (-0 folded into +0, NaN above all), and back
-    static __device__ __forceinline__ uint32_t order16(float v)
-    {
-        const uint32_t u = __builtin_bit_cast(uint16_t, (_Float16)(v + 0.0f));
-        return v != v ? 0xffffu : u & 0x8000u ? u ^ 0xffffu : u | 0x8000u;
-    }
-    static __device__ __forceinline__ float value16(uint32_t o)
-    {
-        return o == 0xffffu ? NAN : (float)__builtin_bit_cast(_Float16, (uint16_t)(o & 0x8000u ? o & 0x7fffu : o ^ 0xffffu));
-    }
-    static __device__ __forceinline__ void unpack(u32x4 w, float *v)
-    {
-        const f16x8 h = __builtin_bit_cast(f16x8, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
-    }
-    static __device__ __forceinline__ u32x4 pack(const float *v)
-    {
-        f16x8 h;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i];
-        return __builtin_bit_cast(u32x4, h);
-    }
-};
-struct BF16 {
-    using raw = uint16_t;
-    static __device__ __forceinline__ u32x4 none() { return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
-    static constexpr int VEC = 8;
-    static __device__ __forceinline__ float get(raw v) { return __uint_as_float((uint32_t)v << 16); }
-    static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(raw, (__bf16)v); }
-    static __device__ __forceinline__ uint32_t order16(float v) { return v != v ? 0xffffu : f32_ordered(v) >> 16; }
-    static __device__ __forceinline__ float value16(uint32_t o)
-    {
-        return o == 0xffffu ? NAN : __uint_as_float((o & 0x8000u ? o & 0x7fffu : o ^ 0xffffu) << 16);
-    }
-    static __device__ __forceinline__ void unpack(u32x4 w, float *v)
-    {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-    static __device__ __forceinline__ u32x4 pack(const float *v)
-    {
-        f32x8 f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = v[i];
-        return __builtin_bit_cast(u32x4, __builtin_convertvector(f, bf16x8));
-    }
-};
-// PASSING: data that passes by once goes around the caches.
-template <class E, bool PASSING = false>
-__device__ __forceinline__ u32x4 load_raw(const typename E::raw *p)
-{
-    typedef typename Unaligned<u32x4, sizeof(typename E::raw)>::type mem;
-    return PASSING ? __builtin_nontemporal_load((const mem *)p) : *(const mem *)p;
-}
-template <class E, bool PASSING = false>
-__device__ __forceinline__ void store_raw(typename E::raw *p, u32x4 v)
-{
-    typedef typename Unaligned<u32x4, sizeof(typename E::raw)>::type mem;
-    if (PASSING) __builtin_nontemporal_store(v, (mem *)p);
-    else *(mem *)p = v;
-}
-
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
-__device__ __forceinline__ float vmax3(float a, float b, float c)
-{
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-
-// ------------------------------------------------------------------------------------------
-// reductions over a wave (DPP) and a block
-// ------------------------------------------------------------------------------------------
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp_f(float old, float x)
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(x), CTRL, ROWS, 0xf, false));
-}
-// x of the wave's lanes combined in lane 63 and handed to all; `none` is the operation's neutral value
-template <class Op>
-__device__ __forceinline__ float wave_reduce(float x, float none, Op op)
-{
-    x = op(x, dpp_f<0x111, 0xf>(none, x));       // row_shr:1
-    x = op(x, dpp_f<0x112, 0xf>(none, x));       // row_shr:2
-    x = op(x, dpp_f<0x114, 0xf>(none, x));       // row_shr:4
-    x = op(x, dpp_f<0x118, 0xf>(none, x));       // row_shr:8
-    x = op(x, dpp_f<0x142, 0xa>(none, x));       // row_bcast:15 into rows 1 and 3
-    x = op(x, dpp_f<0x143, 0xc>(none, x));       // row_bcast:31 into rows 2 and 3
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
-}
-__device__ __forceinline__ float wave_max(float x) { return wave_reduce(x, -INFINITY, [](float a, float b) { return vmax(a, b); }); }
-__device__ __forceinline__ float wave_sum(float x) { return wave_reduce(x, 0.0f, [](float a, float b) { return a + b; }); }
 
 constexpr uint32_t TOP_CAP = 1024;               // candidates of a row's top classes
 constexpr uint32_t MAX_WAVES = 16;
@@ -185,15 +48,10 @@ template <int NT>
 __device__ __forceinline__ float block_max(float v, LogitsLds &sh) { return block_reduce<NT>(v, -INFINITY, sh, [](float a, float b) { return vmax(a, b); }); }
 template <int NT>
 __device__ __forceinline__ float block_sum(float v, LogitsLds &sh) { return block_reduce<NT>(v, 0.0f, sh, [](float a, float b) { return a + b; }); }
+
 // ------------------------------------------------------------------------------------------
 // softmax statistics of a row
 // ------------------------------------------------------------------------------------------
-struct RowStats {
-    float m;             // largest logit; -inf: every logit is -inf (an empty row); NaN: the row holds a NaN or +inf
-    float l2;            // log2 of the sum
-    float ent;           // entropy in nats
-};
-
 // One thread's share of a row in one pass: maximum m, s = sum 2^(x c - mc) and u = sum 2^(x c - mc) (x c - mc), mc = m c as
 // rounded (nmc = -mc).  The fused multiply-add rounds x c - mc once, and join() takes the rounding of mc out again.
 struct Running {
@@ -665,25 +523,6 @@ __device__ __forceinline__ void top_classes(Resident<E, NT> &r, const typename E
 // ------------------------------------------------------------------------------------------
 // scores
 // ------------------------------------------------------------------------------------------
-struct ScoreArgs {
-    const void *logits;
-    size_t rows, stride;
-    uint32_t C, k;
-    float c, inv_t;
-    const int32_t *labels;
-    float *logprobs, *entropy, *top_logprobs;
-    int32_t *top_labels;
-    float4 *stats;
-    uint32_t segs, seg;                          // a row's classes go to `segs` blocks, `seg` (a multiple of 8) to each
-    float4 *part;                                // [rows, segs] shares of a split row
-    uint64_t *part_key;                          // [rows, segs, k]
-};
-
-template <class E>
-__device__ __forceinline__ float logprob_of(const ScoreArgs &a, const RowStats &st, float v)
-{
-    return st.m == -INFINITY ? -INFINITY : (v - st.m) * a.inv_t - LN2 * st.l2;
-}
 // The given label's logit, fetched by one thread in two steps so that neither load is waited for at the row's end.
 struct Label {
     uint32_t id;
@@ -921,18 +760,6 @@ __device__ __forceinline__ void write_grad(const RowStats &st, float ga, float g
     if (threadIdx.x < span.edges) out[span.edge(threadIdx.x)] = E::put(value(E::get(x[span.edge(threadIdx.x)])));
 }
 
-struct ScoreGradArgs {
-    const void *logits;
-    size_t rows, stride;
-    uint32_t C, k;
-    float c, inv_t;
-    const int32_t *labels, *top_labels;
-    const float4 *stats;
-    const float *up_logprobs, *up_entropy, *up_top;
-    void *grad;
-    uint32_t segs, seg;
-};
-
 template <class E, int NT, bool ENT>
 __global__ __launch_bounds__(NT) void score_grad_kernel(ScoreGradArgs a)
 {
@@ -981,24 +808,6 @@ __global__ __launch_bounds__(NT) void score_grad_kernel(ScoreGradArgs a)
 // ------------------------------------------------------------------------------------------
 // distillation
 // ------------------------------------------------------------------------------------------
-struct DistillArgs {
-    const void *logits;
-    size_t rows, stride;
-    uint32_t C, K;
-    float c, t, inv_t, scale;
-    int bucket;
-    const float *teacher;
-    const int32_t *ids;
-    const float *weights;
-    float *out_rows;
-    float4 *stats;
-    const float *up;
-    int up_rows;
-    void *grad;
-    uint32_t segs, seg;
-    float4 *part;                                // [rows, segs] shares of a split row
-};
-
 // The list of one row.  Renormalised: q = softmax of the teacher's values over the listed classes, and the statistics describe all of
 // the student's classes.  Bucket: q = exp(teacher), the teacher's remaining mass q0 = 1 - sum q against the student's mass p0
 // off the list, and the statistics describe the classes OFF the list; all classes follow by adding the listed ones, so neither
@@ -1031,15 +840,6 @@ struct ListEntries {
         }
     }
 };
-
-// exp(t) to about 2^-23 relative for t <= 0: the product with log2(e) in two parts
-__device__ __forceinline__ float exp_split(float t)
-{
-    const float hi = t * LOG2E;
-    if (!(hi > -150.0f)) return t != t ? t : 0.0f;
-    const float lo = __builtin_fmaf(t, LOG2E, -hi) + t * 1.925963033500e-08f;      // LOG2E is log2(e) less that
-    return exp2_hw(hi) * __builtin_fmaf(lo, LN2, 1.0f);
-}
 
 // Fills sh.id (first entries of their classes; -1 otherwise), sh.val (a class's q, summed over its entries), sh.x (the student's
 // logits there), sh.q and sh.logq (by entry) and sh.sum: sum q, q0, and for the bucket the listed classes' maximum and sum about it.
@@ -1375,401 +1175,6 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(DistillArgs a)
     }
 }
 
-// ------------------------------------------------------------------------------------------
-// short rows: L neighbouring lanes hold a row in registers
-// ------------------------------------------------------------------------------------------
-// A block a row wastes itself on rows of a detector's 80 or 90 classes (392 832 of them took 4.3 ms).  Here lane l of a group of L
-// keeps the S vectors l, l + L, .. of its row, so a row is read once whatever is computed from it, a sum is two (L = 4) to six
-// lane exchanges, and no barrier is needed.  S is the exact number of steps, so only the last one looks at the row's end.  The last vector of a row that is no multiple of a vector is read (and
-// written) back from the row's end, its first values counting as dropped: no access leaves the row.
-constexpr int SHORT_THREADS = 256;
-template <class E>
-constexpr int SHORT_STEPS = E::VEC == 4 ? 6 : 4;              // 24 or 32 values a lane
-
-template <int L>
-__device__ __forceinline__ float group_max(float x)
-{
-    x = vmax(x, dpp_f<0xB1, 0xf>(x, x));                     // quad_perm [1,0,3,2]
-    x = vmax(x, dpp_f<0x4E, 0xf>(x, x));                     // quad_perm [2,3,0,1]
-    if (L >= 8) x = vmax(x, dpp_f<0x141, 0xf>(x, x));       // row_half_mirror
-    if (L >= 16) x = vmax(x, dpp_f<0x140, 0xf>(x, x));       // row_mirror
-    if (L >= 32) x = vmax(x, __shfl_xor(x, 16));
-    if (L >= 64) x = vmax(x, __shfl_xor(x, 32));
-    return x;
-}
-template <int L>
-__device__ __forceinline__ float group_sum(float x)
-{
-    x += dpp_f<0xB1, 0xf>(x, x);
-    x += dpp_f<0x4E, 0xf>(x, x);
-    if (L >= 8) x += dpp_f<0x141, 0xf>(x, x);
-    if (L >= 16) x += dpp_f<0x140, 0xf>(x, x);
-    if (L >= 32) x += __shfl_xor(x, 16);
-    if (L >= 64) x += __shfl_xor(x, 32);
-    return x;
-}
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_u(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false); }
-template <int L, class Op>
-__device__ __forceinline__ uint32_t group_fold(uint32_t x, Op op)
-{
-    x = op(x, dpp_u<0xB1>(x));
-    x = op(x, dpp_u<0x4E>(x));
-    if (L >= 8) x = op(x, dpp_u<0x141>(x));
-    if (L >= 16) x = op(x, dpp_u<0x140>(x));
-    if (L >= 32) x = op(x, (uint32_t)__shfl_xor(x, 16));
-    if (L >= 64) x = op(x, (uint32_t)__shfl_xor(x, 32));
-    return x;
-}
-
-template <class E, int L, int S>
-struct ShortRow {
-    static constexpr int VEC = E::VEC, PV = S * VEC;
-    static constexpr bool TINY = L == 4 && S == 1;           // the only variant that meets rows shorter than a vector
-    using raw = typename E::raw;
-    float v[PV];
-    uint32_t lane, C;
-
-    __device__ __forceinline__ ShortRow(uint32_t classes) : lane(threadIdx.x % L), C(classes)
-    {
-        asm volatile("" : "+v"(lane));                       // what is computed from it is not kept from row to row
-    }
-    __device__ __forceinline__ bool tiny() const { return TINY && C < VEC; }
-    __device__ __forceinline__ uint32_t base(int k) const
-    {
-        const uint32_t at = ((uint32_t)k * L + lane) * VEC;
-        if (tiny()) return 0;
-        return k < S - 1 || at < C - VEC ? at : C - VEC;
-    }
-    // leading values of the last step that belong to another vector or, past the row's end, to nobody
-    __device__ __forceinline__ uint32_t drop() const { return ((S - 1) * L + lane) * VEC - base(S - 1); }
-    __device__ __forceinline__ bool counts(int k, int e) const
-    {
-        if (tiny()) return lane == 0 && (uint32_t)e < C;
-        return k < S - 1 || (uint32_t)e >= drop();
-    }
-
-    __device__ __forceinline__ void load(const raw *x)
-    {
-        if (!tiny()) {
-            u32x4 w[S];
-#pragma unroll
-            for (int k = 0; k < S; ++k) w[k] = load_raw<E>(x + base(k));
-#pragma unroll
-            for (int k = 0; k < S; ++k) E::unpack(w[k], v + k * VEC);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = counts(0, e) ? E::get(x[e]) : -INFINITY;
-        }
-    }
-    // f(k, e, value of v[k * VEC + e]); values that do not count are handed over as -inf
-    template <class F>
-    __device__ __forceinline__ void each(F f) const
-    {
-#pragma unroll
-        for (int k = 0; k < S; ++k)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) f(k, e, counts(k, e) ? v[k * VEC + e] : -INFINITY);
-    }
-    // out[class] = f(k, e, value); a dropped value is written too, with what its own lane writes there
-    template <class F>
-    __device__ __forceinline__ void store(raw *out, F f) const
-    {
-        if (!tiny()) {
-#pragma unroll
-            for (int k = 0; k < S; ++k) {
-                float g[VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) g[e] = f(k, e, v[k * VEC + e]);
-                if (k < S - 1 || drop() < VEC) store_raw<E>(out + base(k), E::pack(g));
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (counts(0, e)) out[e] = E::put(f(0, e, v[e]));
-        }
-    }
-    __device__ __forceinline__ void zero(raw *out) const { store(out, [](int, int, float) { return 0.0f; }); }
-};
-
-// Statistics of the values; a NaN comes through the sum, a row without probability has sum 0.
-template <int L, bool ENT, class Each>
-__device__ __forceinline__ RowStats short_stats(float c, Each each)
-{
-    float m = -INFINITY;
-    each([&](int, int, float x) { m = vmax(m, x); });
-    m = group_max<L>(m);
-    const float about = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f, u = 0.0f;
-    each([&](int, int, float x) {
-        const float t = (x - about) * c, e = exp2_hw(t);
-        s += e;
-        if (ENT) u = __builtin_fmaf(e, vmax(t, T_FLOOR), u);
-    });
-    s = group_sum<L>(s);
-    if (s == 0.0f) return {-INFINITY, -INFINITY, 0.0f};
-    if (!(s < INFINITY)) return {NAN, NAN, NAN};
-    const float l2 = log2_hw(s);
-    return {m, l2, ENT ? LN2 * (l2 - group_sum<L>(u) / s) : 0.0f};
-}
-
-template <class E, int L, int S>
-__global__ __launch_bounds__(SHORT_THREADS) void score_short_kernel(ScoreArgs a)
-{
-    using Row = ShortRow<E, L, S>;
-    constexpr uint32_t RB = SHORT_THREADS / L;
-    for (size_t row = (size_t)blockIdx.x * RB + threadIdx.x / L; row < a.rows; row += (size_t)gridDim.x * RB) {
-        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        Row r(a.C);
-        r.load(x);
-        const RowStats st = short_stats<L, true>(a.c, [&](auto f) { r.each(f); });
-        if (r.lane == 0) {
-            if (a.logprobs) {
-                const uint32_t lab = (uint32_t)a.labels[row];
-                a.logprobs[row] = lab < a.C ? logprob_of<E>(a, st, E::get(x[lab])) : 0.0f;
-            }
-            if (a.entropy) a.entropy[row] = st.ent;
-            if (a.stats) a.stats[row] = make_float4(st.m, st.l2, st.ent, 0.0f);
-        }
-        if (a.k == 0) continue;
-        // One round a class: the largest value left, the lowest class that has it; 0 stands for a value that is gone.  A 16-bit value
-        // and its class make one number, so that there the maximum names the class and no two are equal.
-        constexpr bool PAIR = Row::VEC == 8;
-        uint32_t o[Row::PV];
-#pragma unroll
-        for (int i = 0; i < Row::PV; ++i) {
-            const int k = i / Row::VEC, e = i % Row::VEC;
-            const float v = r.v[i];
-            if constexpr (PAIR) o[i] = (E::order16(v) << 16) | (0xffffu - (r.base(k) + e));
-            else o[i] = v != v ? 0xffffffffu : f32_ordered(v);
-            if (!r.counts(k, e)) o[i] = 0;
-        }
-        float keep_lp = 0.0f;
-        int32_t keep_id = 0;
-        for (uint32_t round = 0; round < a.k; ++round) {
-            uint32_t best = 0, win = 0xffffffffu;
-#pragma unroll
-            for (int i = 0; i < Row::PV; ++i) best = o[i] > best ? o[i] : best;
-            best = group_fold<L>(best, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
-            float v;
-            if constexpr (PAIR) {
-                win = 0xffffu - (best & 0xffffu);
-                v = E::value16(best >> 16);
-#pragma unroll
-                for (int i = 0; i < Row::PV; ++i) o[i] = o[i] == best ? 0u : o[i];
-            } else {
-#pragma unroll
-                for (int i = Row::PV - 1; i >= 0; --i) win = o[i] == best ? r.base(i / Row::VEC) + i % Row::VEC : win;
-                win = group_fold<L>(win, [](uint32_t p, uint32_t q) { return p < q ? p : q; });
-#pragma unroll
-                for (int i = 0; i < Row::PV; ++i) o[i] = win - r.base(i / Row::VEC) == (uint32_t)(i % Row::VEC) ? 0u : o[i];
-                v = best == 0xffffffffu ? NAN : f32_unordered(best);
-            }
-            if (round % L == r.lane) {
-                keep_id = (int32_t)win;
-                keep_lp = logprob_of<E>(a, st, v);
-            }
-            if (round % L == L - 1 || round == a.k - 1) {    // L results at a time, side by side
-                const uint32_t at = round - round % L + r.lane;
-                if (at <= round) {
-                    a.top_labels[row * a.k + at] = keep_id;
-                    a.top_logprobs[row * a.k + at] = keep_lp;
-                }
-            }
-        }
-    }
-}
-
-template <class E, int L, int S>
-__global__ __launch_bounds__(SHORT_THREADS) void score_grad_short_kernel(ScoreGradArgs a)
-{
-    using Row = ShortRow<E, L, S>;
-    constexpr uint32_t RB = SHORT_THREADS / L;
-    for (size_t row = (size_t)blockIdx.x * RB + threadIdx.x / L; row < a.rows; row += (size_t)gridDim.x * RB) {
-        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        typename E::raw *out = (typename E::raw *)a.grad + row * a.C;
-        Row r(a.C);
-        r.load(x);
-        const float4 st = a.stats[row];
-        if (st.x == -INFINITY) {
-            r.zero(out);
-            continue;
-        }
-        auto entry = [&](uint32_t j, float &g) -> uint32_t { // class and upstream value of list entry j, the label being the last
-            uint32_t id = a.C;
-            g = 0.0f;
-            if (j < a.k) id = (uint32_t)a.top_labels[row * a.k + j], g = a.up_top[row * a.k + j];
-            else if (a.up_logprobs) id = (uint32_t)a.labels[row], g = a.up_logprobs[row];
-            if (id >= a.C) id = 0xffffffffu, g = 0.0f;
-            return id;
-        };
-        float total = 0.0f, g;
-        for (uint32_t j = 0; j <= a.k; ++j) entry(j, g), total += g;
-        const float gh = a.up_entropy ? a.up_entropy[row] : 0.0f;
-        const float A = -a.inv_t * (total + gh * st.z), B = -a.inv_t * gh * LN2;
-        float grad[Row::PV];
-#pragma unroll
-        for (int i = 0; i < Row::PV; ++i) {
-            const float t = (r.v[i] - st.x) * a.c - st.y;
-            grad[i] = exp2_hw(t) * __builtin_fmaf(B, vmax(t, T_FLOOR), A);
-        }
-        for (uint32_t j = 0; j <= a.k; ++j) {
-            const uint32_t id = entry(j, g);
-            g *= a.inv_t;
-#pragma unroll
-            for (int i = 0; i < Row::PV; ++i) grad[i] += id - r.base(i / Row::VEC) == (uint32_t)(i % Row::VEC) ? g : 0.0f;
-        }
-        r.store(out, [&](int k, int e, float) { return grad[k * Row::VEC + e]; });
-    }
-}
-
-// Losses (out_rows), the gradient (GRAD) or both.  Each group has C words of LDS: -1 for a class off the list, for a listed class
-// first the number of its entry (a class listed twice shows by the entries that do not find theirs), then its q.
-template <class E, int L, int S, bool BUCKET, bool GRAD>
-__global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArgs a)
-{
-    using Row = ShortRow<E, L, S>;
-    constexpr uint32_t RB = SHORT_THREADS / L;
-    constexpr bool LISTED = BUCKET || GRAD;                  // the LDS is needed
-    extern __shared__ __attribute__((aligned(16))) float listed[];
-    const uint32_t pitch = (a.C + 3) & ~3u;
-    float *list = listed + (LISTED ? (threadIdx.x / L) * pitch : 0);
-    for (size_t row = (size_t)blockIdx.x * RB + threadIdx.x / L; row < a.rows; row += (size_t)gridDim.x * RB) {
-        const typename E::raw *x = (const typename E::raw *)a.logits + row * a.stride;
-        typename E::raw *out = (typename E::raw *)a.grad + row * a.C;
-        Row r(a.C);
-        const float w = a.weights ? a.weights[row] : 1.0f;
-        if (w == 0.0f) {                                     // ignored: 0 whatever it holds
-            if (a.out_rows && r.lane == 0) {
-                a.out_rows[row] = 0.0f;
-                if (a.stats) a.stats[row] = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
-            }
-            if (GRAD) r.zero(out);
-            continue;
-        }
-        r.load(x);
-        const float *teacher = a.teacher + row * a.K;
-        const int32_t *ids = a.ids + row * a.K;
-        auto entry = [&](uint32_t j, float &t) -> uint32_t {
-            const uint32_t id = (uint32_t)ids[j];
-            t = id < a.C ? teacher[j] : -INFINITY;
-            return id;
-        };
-        auto fence = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };    // one wave's LDS accesses stay in order
-
-        uint32_t own = 0;                                    // bit i: this lane's i-th entry is its class's first or only one
-        bool twice = false;
-        if (LISTED) {
-            fence();
-            for (uint32_t i = r.lane * 4; i < pitch; i += L * 4) *(float4 *)(list + i) = make_float4(-1.0f, -1.0f, -1.0f, -1.0f);
-            fence();
-            for (uint32_t j = r.lane; j < a.K; j += L)
-                if ((uint32_t)ids[j] < a.C) list[ids[j]] = (float)j;
-            fence();
-            for (uint32_t j = r.lane, i = 0; j < a.K; j += L, ++i) {
-                if ((uint32_t)ids[j] >= a.C) continue;
-                if (list[ids[j]] == (float)j) own |= 1u << i;
-                else twice = true;
-            }
-            fence();
-            twice = group_fold<L>(twice ? 1u : 0u, [](uint32_t p, uint32_t q) { return p | q; }) != 0;
-        }
-        auto off_list = [&](int k, int e) { return list[r.base(k) + e] < 0.0f; };
-        RowStats st;
-        if (BUCKET) {
-            uint32_t bits = 0;                               // the values off the list
-            r.each([&](int k, int e, float) { bits |= (r.counts(k, e) && off_list(k, e) ? 1u : 0u) << (k * Row::VEC + e); });
-            st = short_stats<L, false>(a.c, [&](auto f) { r.each([&](int k, int e, float v) { f(k, e, bits >> (k * Row::VEC + e) & 1u ? v : -INFINITY); }); });
-        } else
-            st = short_stats<L, false>(a.c, [&](auto f) { r.each(f); });
-
-        // the list's terms, as in list_terms()
-        float tm = -INFINITY, tt = 1.0f, mass = 0.0f, q0 = 0.0f, loss = 0.0f;
-        float m = st.m, l2 = st.l2, p0 = 0.0f, t;
-        bool rest = false;
-        if (!BUCKET) {
-            for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), tm = vmax(tm, t);
-            tm = group_max<L>(tm);
-            if (tm > -INFINITY) {
-                tt = 0.0f;
-                for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), tt += exp2_hw((t - tm) * LOG2E);
-                tt = group_sum<L>(tt);
-                mass = 1.0f;
-            }
-        } else {
-            double sum = 0.0;
-            for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), sum += exp((double)t);
-#pragma unroll
-            for (int off = 1; off < L; off <<= 1) sum += __shfl_xor(sum, off);
-            const double left = 1.0 - sum > 0.0 ? 1.0 - sum : 0.0;
-            rest = st.m > -INFINITY;
-            q0 = (float)left;
-            mass = (float)(rest ? sum + left : sum);
-            float top = -INFINITY;
-            for (uint32_t j = r.lane, i = 0; j < a.K; j += L, ++i)
-                if (own >> i & 1u) top = vmax(top, E::get(x[ids[j]]));
-            top = group_max<L>(top);
-            m = vmax(st.m, top);
-            if (m > -INFINITY) {
-                const float off = rest ? exp2_hw((st.m - m) * a.c + st.l2) : 0.0f;
-                float s = 0.0f;
-                for (uint32_t j = r.lane, i = 0; j < a.K; j += L, ++i)
-                    if (own >> i & 1u) s += exp2_hw((E::get(x[ids[j]]) - m) * a.c);
-                s = group_sum<L>(s) + off;
-                l2 = log2_hw(s);
-                p0 = off / s;
-                if (rest && q0 > 0.0f) loss = q0 * (LN2 * log2_hw(q0) - (st.m - m) * a.inv_t - LN2 * (st.l2 - l2));
-            }
-            if (st.m != st.m) m = st.m;
-        }
-        auto q_of = [&](float v) { return BUCKET ? (float)exp((double)v) : tm > -INFINITY ? exp2_hw((v - tm) * LOG2E) / tt : 0.0f; };
-        float terms = 0.0f;
-        for (uint32_t j = r.lane, i = 0; j < a.K; j += L, ++i) {
-            const uint32_t id = entry(j, t);
-            if (id >= a.C) continue;
-            const float q = q_of(t);
-            if (a.out_rows && (q > 0.0f || q != q)) {
-                const float logq = BUCKET ? t : (t - tm) - LN2 * log2_hw(tt);
-                terms += q * (logq - ((E::get(x[id]) - m) * a.inv_t - LN2 * l2));
-            }
-            if (GRAD && (own >> i & 1u)) {
-                float sum = q;
-                if (twice) {
-                    sum = 0.0f;
-                    for (uint32_t n = 0; n < a.K; ++n)
-                        if ((uint32_t)ids[n] == id) sum += q_of(teacher[n]);
-                }
-                list[id] = sum;
-            }
-        }
-        const bool dead = m == -INFINITY;
-        if (a.out_rows) {
-            loss += group_sum<L>(terms);
-            if (r.lane == 0) {
-                a.out_rows[row] = dead ? 0.0f : w * a.t * a.t * loss;
-                if (a.stats) a.stats[row] = make_float4(st.m, st.l2, 0.0f, 0.0f);
-            }
-        }
-        if (GRAD) {
-            fence();
-            if (dead) {
-                r.zero(out);
-            } else {
-                const float coef = w * a.t * a.scale * (a.up ? a.up[a.up_rows ? row : 0] : 1.0f);
-                const float dense = p0 * mass - q0;
-                r.store(out, [&](int k, int e, float v) {
-                    const float b = list[r.base(k) + e];
-                    if (!BUCKET) return coef * (exp2_hw((v - st.m) * a.c - st.l2) * mass - (b < 0.0f ? 0.0f : b));
-                    const bool on = b >= 0.0f || b != b;
-                    const float p = exp2_hw((v - (on ? m : st.m)) * a.c - (on ? l2 : st.l2));
-                    return on ? coef * (p * mass - b) : rest ? coef * dense * p : 0.0f;
-                });
-            }
-            fence();
-        }
-    }
-}
-
 // scale * sum of n floats, in double and in an order fixed by n: block b adds its run of the rows; the last launch adds the blocks.
 constexpr uint32_t SUM_THREADS = 1024, SUM_RUN = 8192, SUM_BLOCKS = 512;
 template <class In, class Out>
@@ -1805,8 +1210,6 @@ static int logits_check(const char *name, const void *logits, int dtype, size_t 
     if ((uintptr_t)logits % (dtype == ODBOX_DTYPE_F32 ? 4 : 2)) return fail(ODBOX_EINVAL, "%s: logits are not aligned to their element", name);
     return 0;
 }
-
-static dim3 work_grid(size_t work) { return dim3((uint32_t)(work < 1u << 20 ? work : 1u << 20)); }
 
 // How a row's classes are dealt out to blocks: whole rows where there are enough of them to fill the chip, else segments of at
 // least 4096 classes so that about `blocks` blocks run.  A segment is a multiple of 8 classes and holds at most `most`.
@@ -1859,50 +1262,6 @@ static void resident_variant(int dtype, uint32_t n, F f)
     else f(std::integral_constant<int, 1024>());
 }
 
-#define LOGITS_LAUNCH(dtype, K_, ...)                                                       \
-    do {                                                                                    \
-        if ((dtype) == ODBOX_DTYPE_F32) { using E = F32; hipLaunchKernelGGL(K_, __VA_ARGS__); } \
-        else if ((dtype) == ODBOX_DTYPE_F16) { using E = F16; hipLaunchKernelGGL(K_, __VA_ARGS__); } \
-        else { using E = BF16; hipLaunchKernelGGL(K_, __VA_ARGS__); }                        \
-    } while (0)
-
-// A short row of nv vectors goes to the smallest group of 4, 8, .. 64 lanes that holds it in SHORT_STEPS steps.
-static int short_limit(int dtype) { return dtype == ODBOX_DTYPE_F32 ? 64 * SHORT_STEPS<F32> * 4 : 64 * SHORT_STEPS<F16> * 8; }
-static dim3 short_grid(size_t rows, int L)
-{
-    const size_t per = SHORT_THREADS / L;
-    return work_grid((rows + per - 1) / per);
-}
-template <int V>
-using Constant = std::integral_constant<int, V>;
-template <class E, int L, int S, class F>
-static void short_lanes(int nv, F f)
-{
-    if (nv > L * SHORT_STEPS<E>) {
-        if constexpr (L < 64) short_lanes<E, 2 * L, SHORT_STEPS<E> / 2 + 1>(nv, f);
-    } else if (nv > L * S) {
-        if constexpr (S < SHORT_STEPS<E>) short_lanes<E, L, S + 1>(nv, f);
-    } else
-        f(E(), Constant<L>(), Constant<S>());
-}
-template <class F>
-static void short_variant(int dtype, int C, F f)
-{
-    if (dtype == ODBOX_DTYPE_F32) short_lanes<F32, 4, 1>((C + 3) / 4, f);
-    else if (dtype == ODBOX_DTYPE_F16) short_lanes<F16, 4, 1>((C + 7) / 8, f);
-    else short_lanes<BF16, 4, 1>((C + 7) / 8, f);
-}
-// The short kernel's selection costs a round for every class on L lanes, the wave's threshold about the same for any k.  Measured
-// (float32, rounds / threshold): 100 000 x 300, k 32 (16 lanes) 162 / 281 us; 40 000 x 600, k 16 (32 lanes) 77 / 97;
-// 20 000 x 1000, k 10 (64 lanes) 49 / 55; 20 000 x 1400, k 20 (64 lanes) 110 / 62.
-static bool score_is_short(int dtype, int C, int k)
-{
-    if (C > short_limit(dtype)) return false;
-    int lanes = 64;
-    short_variant(dtype, C, [&](auto, auto l, auto) { lanes = decltype(l)::value; });
-    return lanes == 4 || k * lanes <= 640;
-}
-
 }  // namespace odbox
 
 using namespace odbox;
@@ -1938,11 +1297,7 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid = work_grid(rows * sp.segs);
     if (score_is_short(dtype, C, top_k)) {
-        short_variant(dtype, C, [&](auto e, auto l, auto n) {
-            using E = decltype(e);
-            constexpr int L = decltype(l)::value, S = decltype(n)::value;
-            hipLaunchKernelGGL((score_short_kernel<E, L, S>), short_grid(rows, L), dim3(SHORT_THREADS), 0, st, a);
-        });
+        score_short(dtype, a, st);
         return launch_status(name);
     }
     if (top_k && sp.seg <= resident(dtype, 64)) LOGITS_LAUNCH(dtype, (score_top_kernel<E, 64>), staying_grid(rows * sp.segs, 64), dim3(64), 0, st, a);
@@ -1971,11 +1326,7 @@ int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, in
                        labels, top_labels, (const float4 *)stats, upstream_logprobs, upstream_entropy, upstream_top, grad, sp.segs, sp.seg};
     const dim3 grid = work_grid(rows * sp.segs);
     if (C <= short_limit(dtype)) {
-        short_variant(dtype, C, [&](auto e, auto l, auto n) {
-            using E = decltype(e);
-            constexpr int L = decltype(l)::value, S = decltype(n)::value;
-            hipLaunchKernelGGL((score_grad_short_kernel<E, L, S>), short_grid(rows, L), dim3(SHORT_THREADS), 0, (hipStream_t)stream, a);
-        });
+        score_grad_short(dtype, a, (hipStream_t)stream);
         return launch_status(name);
     }
     if (upstream_entropy) LOGITS_LAUNCH(dtype, (score_grad_kernel<E, 256, true>), grid, dim3(256), 0, (hipStream_t)stream, a);
@@ -1992,24 +1343,6 @@ static int distill_check(const char *name, const void *logits, int dtype, size_t
     if (rows && (!teacher || !ids)) return fail(ODBOX_EINVAL, "%s: NULL teacher list", name);
     if ((uintptr_t)grad % (dtype == ODBOX_DTYPE_F32 ? 4 : 2)) return fail(ODBOX_EINVAL, "%s: grad is not aligned to its element", name);
     return 0;
-}
-
-static void distill_short(int dtype, int rest, bool grad, const DistillArgs &a, hipStream_t st)
-{
-    const size_t rows = a.rows;
-    short_variant(dtype, (int)a.C, [&](auto e, auto l, auto n) {
-        using E = decltype(e);
-        constexpr int L = decltype(l)::value, S = decltype(n)::value;
-        const size_t lds = (size_t)(SHORT_THREADS / L) * ((a.C + 3) & ~3u) * sizeof(float);
-        const dim3 grid = short_grid(rows, L), block(SHORT_THREADS);
-        if (rest == ODBOX_REST_BUCKET) {
-            if (grad) hipLaunchKernelGGL((distill_short_kernel<E, L, S, true, true>), grid, block, lds, st, a);
-            else hipLaunchKernelGGL((distill_short_kernel<E, L, S, true, false>), grid, block, lds, st, a);
-        } else {
-            if (grad) hipLaunchKernelGGL((distill_short_kernel<E, L, S, false, true>), grid, block, lds, st, a);
-            else hipLaunchKernelGGL((distill_short_kernel<E, L, S, false, false>), grid, block, 0, st, a);
-        }
-    });
 }
 
 size_t odbox_distill_loss_workspace(size_t rows, int C, int K)
