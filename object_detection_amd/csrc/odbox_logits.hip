@@ -1247,6 +1247,14 @@ static bool passes(size_t rows, int C, int dtype, const void *stats)
 {
     return !stats && rows * C > ((size_t)256 << 20) / (dtype == ODBOX_DTYPE_F32 ? 4 : 2);
 }
+// Whole rows that 64 threads could hold in registers get a wave each, which waits for nobody (256 threads / a wave: scores of 100 000 x
+// 2100 bfloat16 189 / 98 us, of 30 000 x 8000 100 / 87; losses of 50 000 x 4000 float32 188 / 119; a bucket step of 50 000 x 4000 bfloat16
+// 719 / 360).
+#define BY_WIDTH(dtype, sp, ...)                                                            \
+    do {                                                                                    \
+        if ((sp).segs == 1 && (sp).seg <= resident(dtype, 64)) { constexpr int NT = 64; __VA_ARGS__; } \
+        else { constexpr int NT = 256; __VA_ARGS__; }                                       \
+    } while (0)
 // Blocks that stay: as many as the 256 CUs hold at four waves a SIMD (128 registers).
 static dim3 staying_grid(size_t work, int nt)
 {
@@ -1302,8 +1310,8 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
     }
     if (top_k && sp.seg <= resident(dtype, 64)) LOGITS_LAUNCH(dtype, (score_top_kernel<E, 64>), staying_grid(rows * sp.segs, 64), dim3(64), 0, st, a);
     else if (top_k) LOGITS_LAUNCH(dtype, (score_top_kernel<E, 256>), staying_grid(rows * sp.segs, 256), dim3(256), 0, st, a);
-    else if (passes(rows, C, dtype, out_stats)) LOGITS_LAUNCH(dtype, (score_kernel<E, 256, true>), grid, dim3(256), 0, st, a);
-    else LOGITS_LAUNCH(dtype, (score_kernel<E, 256, false>), grid, dim3(256), 0, st, a);
+    else if (passes(rows, C, dtype, out_stats)) BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (score_kernel<E, NT, true>), grid, dim3(NT), 0, st, a));
+    else BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (score_kernel<E, NT, false>), grid, dim3(NT), 0, st, a));
     if (sp.segs > 1) LOGITS_LAUNCH(dtype, score_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);
     return launch_status("label_logprobs");
 }
@@ -1329,8 +1337,8 @@ int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, in
         score_grad_short(dtype, a, (hipStream_t)stream);
         return launch_status(name);
     }
-    if (upstream_entropy) LOGITS_LAUNCH(dtype, (score_grad_kernel<E, 256, true>), grid, dim3(256), 0, (hipStream_t)stream, a);
-    else LOGITS_LAUNCH(dtype, (score_grad_kernel<E, 256, false>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    if (upstream_entropy) BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (score_grad_kernel<E, NT, true>), grid, dim3(NT), 0, (hipStream_t)stream, a));
+    else BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (score_grad_kernel<E, NT, false>), grid, dim3(NT), 0, (hipStream_t)stream, a));
     return launch_status("label_logprobs_backward");
 }
 
@@ -1396,14 +1404,14 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
     } else {
         const bool passing = passes(rows, C, dtype, keep);
         if (rest == ODBOX_REST_BUCKET) {
-            if (passing) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true, true>), grid, dim3(256), mask_bytes(256), st, a);
-            else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, true, false>), grid, dim3(256), mask_bytes(256), st, a);
+            if (passing) BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (distill_kernel<E, NT, true, true>), grid, dim3(NT), mask_bytes(NT), st, a));
+            else BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (distill_kernel<E, NT, true, false>), grid, dim3(NT), mask_bytes(NT), st, a));
         } else {
-            if (passing) LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false, true>), grid, dim3(256), 0, st, a);
-            else LOGITS_LAUNCH(dtype, (distill_kernel<E, 256, false, false>), grid, dim3(256), 0, st, a);
+            if (passing) BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (distill_kernel<E, NT, false, true>), grid, dim3(NT), 0, st, a));
+            else BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (distill_kernel<E, NT, false, false>), grid, dim3(NT), 0, st, a));
         }
         if (sp.segs > 1) LOGITS_LAUNCH(dtype, distill_join_kernel<E>, work_grid(rows), dim3(WAVE), 0, st, a);
-        if (grad) LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, 256>), grid, dim3(256), 0, st, a);
+        if (grad) BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, NT>), grid, dim3(NT), 0, st, a));
     }
     if (int rc = launch_status("distill_loss")) return rc;
     if (out_loss) {
@@ -1434,7 +1442,7 @@ int odbox_distill_loss_backward(const void *logits, int dtype, size_t rows, int 
     if (C <= short_limit(dtype)) {
         distill_short(dtype, rest, true, a, (hipStream_t)stream);
     } else
-        LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, 256>), work_grid(rows * sp.segs), dim3(256), 0, (hipStream_t)stream, a);
+        BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (distill_grad_kernel<E, NT>), work_grid(rows * sp.segs), dim3(NT), 0, (hipStream_t)stream, a));
     return launch_status("distill_loss_backward");
 }
 
