@@ -10,8 +10,9 @@ namespace odbox {
 // ------------------------------------------------------------------------------------------
 // A block a row wastes itself on rows of a detector's 80 or 90 classes (392 832 of them took 4.3 ms).  Here lane l of a group of L
 // keeps the S vectors l, l + L, .. of its row, so a row is read once whatever is computed from it, a sum is two (L = 4) to six
-// lane exchanges, and no barrier is needed.  S is the exact number of steps, so only the last one looks at the row's end.  The last vector of a row that is no multiple of a vector is read (and
-// written) back from the row's end, its first values counting as dropped: no access leaves the row.
+// lane exchanges, and no barrier is needed.  S is the exact number of steps, so only the last one looks at the row's end.  The last
+// vector of a row that is no multiple of a vector is read (and written) back from the row's end, its first values counting as
+// dropped: no access leaves the row.
 constexpr int SHORT_THREADS = 256;
 template <class E>
 constexpr int SHORT_STEPS = E::VEC == 4 ? 6 : 4;              // 24 or 32 values a lane
@@ -143,6 +144,8 @@ __device__ __forceinline__ RowStats short_stats(float c, Each each)
     return {m, l2, ENT ? LN2 * (l2 - group_sum<L>(u) / s) : 0.0f};
 }
 
+// 392 832 x 80 float32, five alternatives: 41 us, 3.6 TB/s, bound by the vector unit: five instructions a value and round (maximum,
+// find, remove) where a 16-bit value with its class in one word needs two and a half (bfloat16: 39 us for half the bytes).
 template <class E, int L, int S>
 __global__ __launch_bounds__(SHORT_THREADS) void score_short_kernel(ScoreArgs a)
 {
@@ -210,6 +213,8 @@ __global__ __launch_bounds__(SHORT_THREADS) void score_short_kernel(ScoreArgs a)
     }
 }
 
+// The label's and the alternatives' entries are compared with every value of a lane: two instructions a value and entry, and nothing
+// to write twice.
 template <class E, int L, int S>
 __global__ __launch_bounds__(SHORT_THREADS) void score_grad_short_kernel(ScoreGradArgs a)
 {
@@ -255,6 +260,8 @@ __global__ __launch_bounds__(SHORT_THREADS) void score_grad_short_kernel(ScoreGr
 
 // Losses (out_rows), the gradient (GRAD) or both.  Each group has C words of LDS: -1 for a class off the list, for a listed class
 // first the number of its entry (a class listed twice shows by the entries that do not find theirs), then its q.
+// 392 832 x 80 float16, eight listed: losses 25 us, gradient 38 us (130 MB between them, 3.4 TB/s for the gradient): the chain list, logits there,
+// sums, LDS is waited for more than memory is.
 template <class E, int L, int S, bool BUCKET, bool GRAD>
 __global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArgs a)
 {

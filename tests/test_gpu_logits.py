@@ -56,6 +56,17 @@ def test_scores(rows, C, k, dtype):
         check_scores(x, labels, k, T, M.label_logprobs(x, labels.cuda(), top_k=k, temperature=T))
 
 
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('rows,C', [(1, 1), (9, 90), (5, 700), (7, 2500), (5, 4099), (3, 8009), (1030, 9001), (2, 100003)])
+def test_scores_without_alternatives(rows, C, dtype):
+    x = _make(C, rows, C, dtype)
+    labels = (torch.arange(rows) * 31) % C
+    at = _sample(rows) if rows > 20 else list(range(rows))
+    r = M.label_logprobs(x, labels.cuda(), temperature=1.3)
+    assert r.top_labels is None and r.top_logprobs is None
+    check_scores(x[at], labels[at], 0, 1.3, M.LabelLogprobs(r.logprobs[at], r.entropy[at], None, None))
+
+
 @pytest.mark.parametrize('C', [5, 80, 3001, 70001])
 def test_scores_of_rows_that_lie_apart_transposed_or_once(C):
     x = _make(C, 6, C, BF16, pad=13)
