@@ -171,6 +171,18 @@ def _side(x, dtype, device, shape, what):
     return x.detach().to(device=device, dtype=dtype, non_blocking=True).contiguous()
 
 
+def _class_ids(x, C, device, shape, what):
+    """Class ids that go with the rows, int32.  A wider id that int32 cannot hold is outside [0, C), not what its low bits say."""
+    if not isinstance(x, torch.Tensor):
+        x = torch.as_tensor(x)
+    if x.dtype != torch.int32:
+        if (x.is_floating_point() or x.is_complex()) and x.numel():
+            raise ValueError('%s are %s: class ids are integers' % (what, x.dtype))
+        if x.element_size() > 1:
+            x = x.to(torch.int64).clamp(-1, C)
+    return _side(x, torch.int32, device, shape, what)
+
+
 def _temperature(t):
     t = float(t)
     if not 1e-6 <= t <= 1e6:
@@ -278,7 +290,8 @@ def label_logprobs(logits, labels=None, top_k: int = 0, temperature: float = 1.0
 
     All results are float32.  Rows may lie apart (logits[:, :C] of a padded class axis is read in place).  Differentiable
     w.r.t. the logits through logprobs, entropy and top_logprobs (odbox_label_logprobs_backward; the gradient has the logits'
-    type).  A logit of -inf is a forbidden class; a row of nothing else gives log-probabilities -inf, entropy 0 and no
+    type; inside a graph capture, differentiate w.r.t. a leaf made there, logits.detach().requires_grad_(): a leaf of a live
+    eager graph ties the capture to that graph's stream).  A logit of -inf is a forbidden class; a row of nothing else gives log-probabilities -inf, entropy 0 and no
     gradient; a NaN or +inf makes its row NaN.  On a teacher, `top_logprobs` / `top_labels` are what `distill_loss` takes."""
     x = _logits(logits)
     temperature = _temperature(temperature)
@@ -286,7 +299,7 @@ def label_logprobs(logits, labels=None, top_k: int = 0, temperature: float = 1.0
     if not 0 <= top_k <= min(MAX_TOP, x.shape[-1]):
         raise ValueError('top_k %d is not in 0..min(%d classes, %d)' % (top_k, x.shape[-1], MAX_TOP))
     if labels is not None:
-        labels = _side(labels, torch.int32, x.device, x.shape[:-1], 'labels')
+        labels = _class_ids(labels, x.shape[-1], x.device, x.shape[:-1], 'labels')
     if torch.is_grad_enabled() and x.requires_grad:
         return LabelLogprobs(*_LabelLogprobsFn.apply(x, labels, top_k, temperature))
     with _on(x.device):
@@ -355,7 +368,7 @@ def distill_loss(logits, teacher_logprobs, teacher_labels, temperature: float = 
     rest = q0 (log q0 - log p0).  A row of weight 0 is ignored whatever it holds.
 
     reduction 'sum' (default), 'mean' (over the rows; 0 for none) or anything else (e.g. None): the losses [...] themselves,
-    float32.  Differentiable w.r.t. the logits; return_grad=True instead returns (loss, gradient), the gradient in the
+    float32.  Differentiable w.r.t. the logits (captures: as label_logprobs); return_grad=True instead returns (loss, gradient), the gradient in the
     logits' type from the same call -- one pass over the logits where autograd takes two -- of the reduced loss, or for
     un-reduced losses of each row's loss w.r.t. that row."""
     x = _logits(logits)
@@ -368,7 +381,7 @@ def distill_loss(logits, teacher_logprobs, teacher_labels, temperature: float = 
     K = int(teacher_labels.shape[-1]) if teacher_labels.dim() else 0
     if not 1 <= K <= MAX_TOP:
         raise ValueError('teacher_labels %r: the last axis holds 1..%d classes' % (tuple(teacher_labels.shape), MAX_TOP))
-    ids = _side(teacher_labels, torch.int32, x.device, lead + (K,), 'teacher_labels')
+    ids = _class_ids(teacher_labels, x.shape[-1], x.device, lead + (K,), 'teacher_labels')
     tl = _side(teacher_logprobs, torch.float32, x.device, lead + (K,), 'teacher_logprobs')
     w = None if row_weights is None else _side(row_weights, torch.float32, x.device, lead, 'row_weights')
     per_row = reduction not in ('sum', 'mean')

@@ -638,6 +638,20 @@ def test_inputs_changed_before_the_backward_pass_are_noticed():
         loss.backward()
 
 
+def test_ids_wider_than_int32():
+    x = _make(2, 4, 50, F32)
+    wide = torch.tensor([7, (1 << 32) + 7, -(1 << 63), 1 << 40])
+    fits = torch.tensor([7, -1, -1, -1])
+    a, b = M.label_logprobs(x, wide), M.label_logprobs(x, fits.int().cuda())
+    assert torch.equal(a.logprobs, b.logprobs) and (a.logprobs[1:] == 0).all() and a.logprobs[0] < 0
+    tl = torch.full((4, 2), -1.0)
+    la, lb = (M.distill_loss(x, tl, torch.stack([torch.arange(4), i], -1).cuda(), reduction=None) for i in (wide, fits))
+    assert torch.equal(la, lb)
+    for bad in (torch.zeros(4), torch.zeros(4, device='cuda', dtype=F16)):
+        with pytest.raises(ValueError):
+            M.label_logprobs(x, bad)
+
+
 def test_python_refusals():
     x = torch.zeros(4, 10, device='cuda')
     ids = torch.zeros(4, 3, dtype=torch.int32)

@@ -133,3 +133,14 @@ def test_reference_gradients_against_autograd(bucket):
     grad, = torch.autograd.grad(0.5 * logp[3] + 2.0 * ent - logp[3] + 0.25 * logp[0], x)
     g, _ = R.score_grad(row, 3, 0.5, 2.0, [3, 0], [-1.0, 0.25])
     np.testing.assert_allclose(g, grad.numpy(), atol=1e-13)
+
+
+def test_class_ids_that_int32_cannot_hold_are_outside_the_classes():
+    wide = [3, -1, 10, -100, (1 << 32) + 3, -(1 << 63), (1 << 63) - 1, -(1 << 32)]
+    got = metric._class_ids(torch.tensor(wide), 10, torch.device('cpu'), torch.Size([8]), 'labels')
+    assert got.dtype == torch.int32 and got[0] == 3
+    assert all(not 0 <= v < 10 for v in got[1:].tolist()), got
+    assert metric._class_ids(torch.tensor([200], dtype=torch.uint8), 300, torch.device('cpu'), torch.Size([1]), 'labels').tolist() == [200]
+    for bad in (torch.tensor([1.0]), torch.tensor([1.0], dtype=torch.float16)):
+        with pytest.raises(ValueError):
+            metric._class_ids(bad, 10, torch.device('cpu'), torch.Size([1]), 'labels')
