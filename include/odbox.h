@@ -325,7 +325,7 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
 /* Its gradient, grad [rows, C] of the logits' dtype, contiguous, rounded once:
  *   d logits_i = (1/T) [ sum_j g_j [i = id_j] - p_i (sum_j g_j + gH (log p_i + H)) ]
  * over the label's upstream value and those of the top alternatives (at their fixed classes); each upstream may be NULL.
- * logits, labels, temperature and stats are the forward call's. */
+ * logits, labels, temperature and stats are the forward call's; grad may not overlap the logits. */
 int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, int C, size_t row_stride,
                                   const int32_t *labels /*[rows] or NULL*/, int top_k,
                                   const int32_t *top_labels /*[rows,top_k] or NULL*/, float temperature,
@@ -342,7 +342,7 @@ int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, in
  *   rest = q0 (log q0 - log p0), q0 = max(0, 1 - sum q), p0 = the student's mass off the list; left out where the student has none.
  * row_weights w [rows] or NULL (all 1); a row of weight 0 is ignored: its logits are not read, its loss and gradient are 0.
  * out_rows [rows] or NULL: the row losses.  out_loss [1] or NULL: scale * their sum, summed in a fixed order (not both NULL).
- * grad [rows, C] or NULL: the gradient of scale * the sum, of the logits' dtype, contiguous.
+ * grad [rows, C] or NULL: the gradient of scale * the sum, of the logits' dtype, contiguous; it may not overlap the logits.
  * out_stats [rows, 4] (16-byte aligned, or NULL) is what the backward call needs.
  * workspace: odbox_distill_loss_workspace(rows, C, K) bytes, 16-byte aligned. */
 #define ODBOX_REST_RENORMALISE 0
