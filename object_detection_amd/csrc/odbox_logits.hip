@@ -1249,11 +1249,11 @@ static Split distill_split(size_t rows, uint32_t C)
     return split_rows(rows, C, FILL_BLOCKS, MASK_CLASSES);
 }
 // Logits that nobody reads again (no statistics are kept for a gradient) and that the 256 MB Infinity Cache could not hold are read around
-// the caches: 2048 x 131072 bfloat16 scores 99 -> 92 us, 2048 x 32768 float32 losses 53 -> 49 us.  Ahead of a gradient the same loads cost
+// the caches: 2048 x 131072 bfloat16 scores 99 -> 92 us, 2048 x 32768 float32 losses (256 MB) 51 -> 48 us.  Ahead of a gradient the same loads cost
 // what its second read then misses (1021 x 100003 float16 both ways 126 -> 146 us).
 static bool passes(size_t rows, int C, int dtype, const void *stats)
 {
-    return !stats && rows * C > ((size_t)256 << 20) / (dtype == ODBOX_DTYPE_F32 ? 4 : 2);
+    return !stats && rows * C >= ((size_t)256 << 20) / (dtype == ODBOX_DTYPE_F32 ? 4 : 2);
 }
 // Whole rows that 64 threads could hold in registers get a wave each, which waits for nobody (256 threads / a wave: scores of 100 000 x
 // 2100 bfloat16 189 / 98 us, of 30 000 x 8000 100 / 87; losses of 50 000 x 4000 float32 188 / 119; a bucket step of 50 000 x 4000 bfloat16
