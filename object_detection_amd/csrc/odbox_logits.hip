@@ -1018,8 +1018,8 @@ __device__ __forceinline__ void listed_grad(const DistillArgs &a, float coef, co
 constexpr uint32_t MASK_CLASSES = 262144;        // of a bucket segment: 32 KB of mask
 
 // Losses, one block per row or per segment of a row: the row streams by.  2048 x 32768 float32: 46 us, 5.5 TB/s.  The bucket's mask costs a
-// word of LDS for every 32 values of a thread and, where a wave has a listed class in them, two more instructions a value:
-// 2048 x 131072 bfloat16, 64 listed 117 us.
+// word of LDS for every 32 values of a thread and, where a wave has a listed class in them, three more instructions a value, which hide
+// behind the reads: 2048 x 131072 bfloat16, 64 listed 117 us.  (Eight blocks a CU for it: 312 -> 326 us with the gradient.)
 template <class E, int NT, bool BUCKET, bool PASSING>
 __global__ __launch_bounds__(NT, BUCKET ? 6 : 8) void distill_kernel(DistillArgs a)
 {
@@ -1248,13 +1248,13 @@ static Split distill_split(size_t rows, uint32_t C)
 {
     return split_rows(rows, C, FILL_BLOCKS, MASK_CLASSES);
 }
-// Logits that nobody reads again (no statistics are kept for a gradient) and that the 256 MB Infinity Cache could not hold are read around
-// the caches: 2048 x 131072 bfloat16 scores 99 -> 92 us, 2048 x 32768 float32 losses (256 MB) 51 -> 48 us.  Ahead of a gradient the same loads cost
-// what its second read then misses (1021 x 100003 float16 both ways 126 -> 146 us).
-static bool passes(size_t rows, int C, int dtype, const void *stats)
-{
-    return !stats && rows * C >= ((size_t)256 << 20) / (dtype == ODBOX_DTYPE_F32 ? 4 : 2);
-}
+// Logits that the 256 MB Infinity Cache could not hold are read around the caches when nobody reads them again (no statistics are kept for
+// a gradient): 2048 x 131072 bfloat16 scores 99 -> 92 us, 2048 x 32768 float32 losses (256 MB) 51 -> 48 us.  Ahead of a gradient the same
+// loads cost what its second read then misses (1021 x 100003 float16 scores both ways 126 -> 146 us, 4600 rows still 590 -> 618); losses
+// gain where the cache holds little of them: both ways 300 x 1000003 bfloat16 (600 MB) 376 -> 384 us, 3600 x 100003 (720 MB) 455 ->
+// 442, 4000 x 131072 605 -> 554.
+static bool passes(size_t rows, int C, int dtype, size_t from) { return rows * C >= from / (dtype == ODBOX_DTYPE_F32 ? 4 : 2); }
+constexpr size_t PASS_ONCE = (size_t)256 << 20, PASS_AGAIN = (size_t)640 << 20;
 // Whole rows that 64 threads could hold in registers get a wave each, which waits for nobody (256 threads / a wave: scores of 100 000 x
 // 2100 bfloat16 189 / 98 us, of 30 000 x 8000 100 / 87; losses of 50 000 x 4000 float32 188 / 119; a bucket step of 50 000 x 4000 bfloat16
 // 719 / 360).
@@ -1318,7 +1318,7 @@ int odbox_label_logprobs(const void *logits, int dtype, size_t rows, int C, size
     }
     if (top_k && sp.seg <= resident(dtype, 64)) LOGITS_LAUNCH(dtype, (score_top_kernel<E, 64>), staying_grid(rows * sp.segs, 64), dim3(64), 0, st, a);
     else if (top_k) LOGITS_LAUNCH(dtype, (score_top_kernel<E, 256>), staying_grid(rows * sp.segs, 256), dim3(256), 0, st, a);
-    else if (passes(rows, C, dtype, out_stats)) BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (score_kernel<E, NT, true>), grid, dim3(NT), 0, st, a));
+    else if (!out_stats && passes(rows, C, dtype, PASS_ONCE)) BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (score_kernel<E, NT, true>), grid, dim3(NT), 0, st, a));
     else BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (score_kernel<E, NT, false>), grid, dim3(NT), 0, st, a));
     if (sp.segs > 1) LOGITS_LAUNCH(dtype, score_join_kernel<E>, work_grid(rows), dim3(JOIN_THREADS), 0, st, a);
     return launch_status("label_logprobs");
@@ -1410,7 +1410,7 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
             else LOGITS_LAUNCH(dtype, (distill_fused_kernel<E, NT, false>), staying_grid(rows, NT), dim3(NT), 0, st, a);
         });
     } else {
-        const bool passing = passes(rows, C, dtype, keep);
+        const bool passing = passes(rows, C, dtype, keep ? PASS_AGAIN : PASS_ONCE);
         if (rest == ODBOX_REST_BUCKET) {
             if (passing) BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (distill_kernel<E, NT, true, true>), grid, dim3(NT), mask_bytes(NT), st, a));
             else BY_WIDTH(dtype, sp, LOGITS_LAUNCH(dtype, (distill_kernel<E, NT, true, false>), grid, dim3(NT), mask_bytes(NT), st, a));

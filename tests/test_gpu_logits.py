@@ -446,6 +446,25 @@ def test_more_logits_than_the_caches_hold(rest):
     check_score_grad(x[at], labels[at], 0, 1.0, np.ones(len(at)), np.zeros(len(at)), np.zeros((len(at), 1)), [[0]] * len(at), g[at])
 
 
+@pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
+def test_gradient_of_more_logits_than_the_caches_hold(rest):
+    """A gradient has the bits that its rows give in a smaller call."""
+    rows, C, part = 82000, 4100, 2048                           # 672 MB
+    x = _make(5, part, C, BF16).repeat(41, 1)[:rows]
+    tl, ids = _list(5, x[:part], 5, 1.0)
+    tl, ids = tl.repeat(41, 1)[:rows], ids.repeat(41, 1)[:rows]
+
+    def grad(n):
+        leaf = x[:n].requires_grad_()
+        loss = M.distill_loss(leaf, tl[:n], ids[:n], rest=rest, reduction=None)
+        return loss, torch.autograd.grad(loss.sum(), leaf)[0]
+    l0, g0 = grad(part)
+    l, g = grad(rows)
+    for r in range(0, rows, part):
+        n = min(part, rows - r)
+        assert torch.equal(l[r:r + n], l0[:n]) and torch.equal(g[r:r + n], g0[:n]), r
+
+
 def test_results_do_not_change_from_call_to_call():
     x = _make(1, 40, 30011, BF16)
     x = (x.float() * 4).round().div(4).to(BF16)                 # many ties
