@@ -143,6 +143,7 @@ struct RowStats {
     float m;             // largest logit; -inf: every logit is -inf (an empty row); NaN: the row holds a NaN or +inf
     float l2;            // log2 of the sum
     float ent;           // entropy in nats
+    float s;             // the sum itself
 };
 
 struct ScoreArgs {
@@ -202,6 +203,31 @@ __device__ __forceinline__ float exp_split(float t)
     if (!(hi > -150.0f)) return t != t ? t : 0.0f;
     const float lo = __builtin_fmaf(t, LOG2E, -hi) + t * 1.925963033500e-08f;      // LOG2E is log2(e) less that
     return exp2_hw(hi) * __builtin_fmaf(lo, LN2, 1.0f);
+}
+
+// log(1 + x) for |x| <= 1/2 or 0 <= x <= 1, as exact near 0 as elsewhere: the rounding of 1 + x is taken out by x / ((1 + x) - 1)
+__device__ __forceinline__ float log1p_hw(float x)
+{
+    const float u = 1.0f + x;
+    return u == 1.0f ? x : LN2 * log2_hw(u) * (x / (u - 1.0f));
+}
+
+// The bucket of a row: p0 and q0, the student's and the teacher's mass off the list.  Where the list holds little both are near 1, and loss and
+// gradient live on their difference: there they come from on / off and sum q, which are small, and not from what those leave of 1.
+struct BucketTerms {
+    float dense;         // p0 (sum q + q0) - q0
+    float rest;          // q0 (log q0 - log p0)
+};
+// on, off: the student's sums on and off the list; log_far: log p0 from maxima and logarithms, for a p0 that float32 does not reach
+__device__ __forceinline__ BucketTerms bucket_terms(float on, float off, float sum_q, float q0, float log_far)
+{
+    const float s = on + off, p0 = off / s;
+    BucketTerms r;
+    r.dense = q0 > 0.0f && p0 > 0.5f ? sum_q - on / s : p0 * (sum_q + q0) - q0;
+    const float log_q0 = sum_q < 0.5f ? log1p_hw(-sum_q) : LN2 * log2_hw(q0);
+    const float log_p0 = p0 > 0.5f ? -log1p_hw(on / off) : p0 > 1e-30f ? LN2 * log2_hw(p0) : log_far;
+    r.rest = q0 > 0.0f ? q0 * (log_q0 - log_p0) : 0.0f;
+    return r;
 }
 
 #define LOGITS_LAUNCH(dtype, K_, ...)                                                       \

@@ -118,7 +118,7 @@ __device__ __forceinline__ bool row_ok(const float3 &j) { return j.y > 0.0f && j
 __device__ __forceinline__ RowStats stats_of(const float3 &j)
 {
     const float l2 = log2_hw(j.y);
-    return {j.x, l2, LN2 * (l2 - j.z / j.y)};
+    return {j.x, l2, LN2 * (l2 - j.z / j.y), j.y};
 }
 
 // Two passes over the row by the whole block, for the rows that are not row_ok; the classes among the K of sh.id are left out.
@@ -140,8 +140,8 @@ __device__ __attribute__((noinline)) RowStats careful_stats(const typename E::ra
     }
     m = block_max<NT>(m, sh);
     bad = block_max<NT>(bad, sh);
-    if (bad != 0.0f) return {NAN, NAN, NAN};
-    if (m == -INFINITY) return {m, -INFINITY, 0.0f};
+    if (bad != 0.0f) return {NAN, NAN, NAN, NAN};
+    if (m == -INFINITY) return {m, -INFINITY, 0.0f, 0.0f};
     float s = 0.0f, u = 0.0f;
     for (uint32_t i = threadIdx.x; i < C; i += NT) {
         if (skip(i)) continue;
@@ -152,7 +152,7 @@ __device__ __attribute__((noinline)) RowStats careful_stats(const typename E::ra
     s = block_sum<NT>(s, sh);
     u = block_sum<NT>(u, sh);
     const float l2 = log2_hw(s);
-    return {m, l2, LN2 * (l2 - u / s)};
+    return {m, l2, LN2 * (l2 - u / s), s};
 }
 
 // n classes of a row as seen by 16-byte loads: `head` classes up to the first boundary, nvec vectors, the rest.  Head and rest, fewer than
@@ -774,7 +774,7 @@ __global__ __launch_bounds__(NT) void score_grad_kernel(ScoreGradArgs a)
         const typename E::raw *x = (const typename E::raw *)a.logits + p.row * a.stride;
         typename E::raw *out = (typename E::raw *)a.grad + p.row * a.C + p.first;
         const float4 f = a.stats[p.row];
-        const RowStats st = {f.x, f.y, f.z};
+        const RowStats st = {f.x, f.y, f.z, 0.0f};
         if (st.m == -INFINITY) {                             // an empty row has constant outputs
             zero_classes<E, NT>(out, p.n);
             continue;
@@ -950,11 +950,12 @@ __device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, const RowS
     r.m = vmax(st.m, top);
     r.l2 = -INFINITY;
     if (r.m > -INFINITY) {
-        const float off = rest ? exp2_hw((st.m - r.m) * a.c + st.l2) : 0.0f;
-        const float s = (top > -INFINITY ? s_on * exp2_hw((top - r.m) * a.c) : 0.0f) + off;
-        r.l2 = log2_hw(s);
-        r.dense = off / s * r.mass - q0;
-        if (rest && q0 > 0.0f) r.rest = q0 * (LN2 * log2_hw(q0) - (st.m - r.m) * a.inv_t - LN2 * (st.l2 - r.l2));
+        const float off = rest ? st.s * exp2_hw((st.m - r.m) * a.c) : 0.0f;
+        const float on = top > -INFINITY ? s_on * exp2_hw((top - r.m) * a.c) : 0.0f;
+        r.l2 = log2_hw(on + off);
+        const BucketTerms b = bucket_terms(on, off, mass, q0, (st.m - r.m) * a.inv_t + LN2 * (st.l2 - r.l2));
+        r.dense = b.dense;
+        if (rest) r.rest = b.rest;
         if (q0 != q0) r.rest = q0;
     }
     if (st.m != st.m || s_on != s_on) r.m = NAN;
@@ -993,7 +994,7 @@ __device__ __forceinline__ void loss_out(const DistillArgs &a, size_t row, float
     terms = wave_sum(terms) + r.rest;
     if (threadIdx.x == 0) {
         a.out_rows[row] = r.m == -INFINITY ? 0.0f : w * a.t * a.t * terms;
-        if (a.stats) a.stats[row] = make_float4(st.m, st.l2, 0.0f, 0.0f);
+        if (a.stats) a.stats[row] = make_float4(st.m, st.l2, st.s, 0.0f);
     }
 }
 __device__ __forceinline__ void ignored_out(const DistillArgs &a, size_t row)
@@ -1170,7 +1171,7 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(DistillArgs a)
         if (threadIdx.x < WAVE) load_and_prepare<E>(a, p.row, x, sh);
         __syncthreads();
         const float4 f = a.stats[p.row];
-        const RowStats st = {f.x, f.y, 0.0f};
+        const RowStats st = {f.x, f.y, 0.0f, f.z};
         const ListTerms t = list_terms(a, st, sh);
         const float coef = weight * a.t * a.scale * (a.up ? a.up[a.up_rows ? p.row : 0] : 1.0f);
         if (t.m == -INFINITY) {

@@ -138,10 +138,10 @@ __device__ __forceinline__ RowStats short_stats(float c, Each each)
         if (ENT) u = __builtin_fmaf(e, vmax(t, T_FLOOR), u);
     });
     s = group_sum<L>(s);
-    if (s == 0.0f) return {-INFINITY, -INFINITY, 0.0f};
-    if (!(s < INFINITY)) return {NAN, NAN, NAN};
+    if (s == 0.0f) return {-INFINITY, -INFINITY, 0.0f, 0.0f};
+    if (!(s < INFINITY)) return {NAN, NAN, NAN, NAN};
     const float l2 = log2_hw(s);
-    return {m, l2, ENT ? LN2 * (l2 - group_sum<L>(u) / s) : 0.0f};
+    return {m, l2, ENT ? LN2 * (l2 - group_sum<L>(u) / s) : 0.0f, s};
 }
 
 // 392 832 x 80 float32, five alternatives: 41 us, 3.6 TB/s, bound by the vector unit: five instructions a value and round (maximum,
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArg
 
         // the list's terms, as in list_terms()
         float tm = -INFINITY, tt = 1.0f, mass = 0.0f, q0 = 0.0f, loss = 0.0f;
-        float m = st.m, l2 = st.l2, p0 = 0.0f, t;
+        float m = st.m, l2 = st.l2, dense = 0.0f, t;
         bool rest = false;
         if (!BUCKET) {
             for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), tm = vmax(tm, t);
@@ -348,14 +348,15 @@ __global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArg
             top = group_max<L>(top);
             m = vmax(st.m, top);
             if (m > -INFINITY) {
-                const float off = rest ? exp2_hw((st.m - m) * a.c + st.l2) : 0.0f;
-                float s = 0.0f;
+                const float off = rest ? st.s * exp2_hw((st.m - m) * a.c) : 0.0f;
+                float on = 0.0f;
                 for (uint32_t j = r.lane, i = 0; j < a.K; j += L, ++i)
-                    if (own >> i & 1u) s += exp2_hw((E::get(x[ids[j]]) - m) * a.c);
-                s = group_sum<L>(s) + off;
-                l2 = log2_hw(s);
-                p0 = off / s;
-                if (rest && q0 > 0.0f) loss = q0 * (LN2 * log2_hw(q0) - (st.m - m) * a.inv_t - LN2 * (st.l2 - l2));
+                    if (own >> i & 1u) on += exp2_hw((E::get(x[ids[j]]) - m) * a.c);
+                on = group_sum<L>(on);
+                l2 = log2_hw(on + off);
+                const BucketTerms b = bucket_terms(on, off, (float)sum, q0, (st.m - m) * a.inv_t + LN2 * (st.l2 - l2));
+                dense = b.dense;
+                if (rest) loss = b.rest;
             }
             if (q0 != q0) loss = q0;
             if (st.m != st.m) m = st.m;
@@ -385,7 +386,7 @@ __global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArg
             loss += group_sum<L>(terms);
             if (r.lane == 0) {
                 a.out_rows[row] = dead ? 0.0f : w * a.t * a.t * loss;
-                if (a.stats) a.stats[row] = make_float4(st.m, st.l2, 0.0f, 0.0f);
+                if (a.stats) a.stats[row] = make_float4(st.m, st.l2, st.s, 0.0f);
             }
         }
         if (GRAD) {
@@ -394,7 +395,6 @@ __global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArg
                 r.zero(out);
             } else {
                 const float coef = w * a.t * a.scale * (a.up ? a.up[a.up_rows ? row : 0] : 1.0f);
-                const float dense = p0 * mass - q0;
                 r.store(out, [&](int k, int e, float v) {
                     const float b = list[r.base(k) + e];
                     if (!BUCKET) return coef * (exp2_hw((v - st.m) * a.c - st.l2) * mass - (b < 0.0f ? 0.0f : b));

@@ -309,6 +309,43 @@ def test_distill_gradient_against_differences(rest):
     assert (grad[0] - want).abs().max() < 2 * h * h / 6 * 4 / T + 4 * 4e-6 / (2 * h)
 
 
+@pytest.mark.parametrize('C', [90, 1400, 11921, 60001])
+@pytest.mark.parametrize('T', [1.0, 4.0])
+def test_bucket_where_student_and_teacher_hardly_differ(C, T):
+    """The list holds little and both masses off it are near 1: the loss is a small difference, and has to come from what is listed.
+
+    Bound.  e = U (4 t + 4 + adds(C) + 4 l2) is a sum's relative error (Row.err over all classes at most `spread`, its largest).  on / off is off
+    by 2 e relative, so log p0 = -log(1 + on / off) by p_on (2 e + 4 U); q by (K + 8 + 4 |log q|) U relative, log q0 by as much of sum q / q0.
+    A listed term by q (q_rel |d| + e + q_rel + 4 U (|log q| + |log p|)), and every product and sum by a few U of its own size."""
+    rows, K = 24, 3
+    g = torch.Generator().manual_seed(C)
+    teacher = torch.randn(rows, C, generator=g).cuda()
+    x = teacher + 0.05 * torch.randn(rows, C, generator=g).cuda()
+    r = M.label_logprobs(teacher, top_k=K, temperature=T)
+    tl, ids = r.top_logprobs, r.top_labels
+    loss, grad = M.distill_loss(x, tl, ids, temperature=T, rest='bucket', reduction=None, return_grad=True)
+    leaf = x.clone().requires_grad_()
+    again, = torch.autograd.grad(M.distill_loss(leaf, tl, ids, temperature=T, rest='bucket'), leaf)
+    xs, t, n = _np(x), _np(tl), ids.cpu().numpy()
+    for i in range(rows):
+        row = R.Row(xs[i], T)
+        want, wg, _, _ = R.distill(row, t[i], n[i], True, 1.0)
+        q, lp = np.exp(t[i]), row.logp[n[i]]
+        q0, p_on, e, U = 1 - q.sum(), row.p[n[i]].sum(), row.err.max(), R.U
+        q_rel = U * (K + 8 + 4 * np.abs(t[i]))
+        mass_err = (q * q_rel).sum() + 2 * U * q.sum()
+        err = (q * (q_rel * np.abs(t[i] - lp) + e + q_rel + 4 * U * (np.abs(t[i]) + np.abs(lp)))).sum()
+        err += p_on * (2 * e + 4 * U) + mass_err / q0 + 8 * U * (abs(np.log(q0)) + abs(np.log(1 - p_on)) + np.abs(q * (t[i] - lp)).sum())
+        R.within(float(loss[i]), want, T * T * err + 4 * U * want, 'loss of row %d' % i)
+        # off the list: T r_i (sum q - p_on)
+        off = np.ones(C, bool)
+        off[n[i]] = False
+        dense = p_on * (2 * e + 4 * U) + mass_err
+        bound = T * row.p[off] / (1 - p_on) * dense + (2 * e + 16 * U) * np.abs(wg[off]) + R.TINY[F32]
+        for got in (grad, again):
+            R.within(_np(got[i])[off], wg[off], bound, 'gradient of row %d' % i)
+
+
 def test_renormalised_list_does_not_see_a_shift_of_the_teacher():
     x = _make(5, 8, 200, F32)
     t = torch.randn(8, 10, generator=torch.Generator().manual_seed(1)).cuda()
