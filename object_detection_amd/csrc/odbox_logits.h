@@ -205,6 +205,34 @@ __device__ __forceinline__ float exp_split(float t)
     return exp2_hw(hi) * __builtin_fmaf(lo, LN2, 1.0f);
 }
 
+// exp(t) for t <= 0 to 2^-51 absolute, for sums that are taken from 1: 2^k exp(r)^2 with |2 r| <= ln(2) / 2, exp(r) by its series up to
+// r^10 / 10! (r^11 / 11! < 2^-53); below -40 it is 0, which is 2^-57 off.  The coefficients are handed over in scalar registers: held from row
+// to row in vector registers, as the compiler and the library's exponential do, they cost the row its own (bucket losses of 2048 x
+// 32768 34 -> 47 us).
+__device__ __forceinline__ double exp_wide(float t)
+{
+    if (!(t > -40.0f)) return t != t ? (double)t : 0.0;
+    const float k = __builtin_rintf(t * LOG2E);
+    const double r = __builtin_fma((double)k, -0.69314718055994530942 / 2, (double)t * 0.5);
+    double e = 1.0 / 3628800;
+    const auto step = [&](double c) {
+        asm volatile("" : "+s"(c));
+        e = __builtin_fma(e, r, c);
+    };
+    asm volatile("" : "+s"(e));
+    step(1.0 / 362880);
+    step(1.0 / 40320);
+    step(1.0 / 5040);
+    step(1.0 / 720);
+    step(1.0 / 120);
+    step(1.0 / 24);
+    step(1.0 / 6);
+    e = __builtin_fma(e, r, 0.5);
+    e = __builtin_fma(e, r, 1.0);
+    e = __builtin_fma(e, r, 1.0);
+    return __builtin_ldexp(e * e, (int)k);
+}
+
 // log(1 + x) for |x| <= 1/2 or 0 <= x <= 1, as exact near 0 as elsewhere: the rounding of 1 + x is taken out by x / ((1 + x) - 1)
 __device__ __forceinline__ float log1p_hw(float x)
 {

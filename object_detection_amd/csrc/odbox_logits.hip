@@ -873,10 +873,10 @@ __device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEnt
         for (int h = 0; h < 2; ++h) {
             q[h] = on[h] ? exp_split(en.t[h]) : 0.0f;
             logq[h] = en.t[h];
-            sum += (double)q[h];
+            if (on[h]) sum += exp_wide(en.t[h]);
         }
         for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
-        const double left = 1.0 - sum;           // in double: where the list holds nearly everything, little is left of it
+        const double left = 1.0 - sum;           // exponentials and sum in double: where the list holds nearly everything, little is left of it
         q0 = left > 0.0 ? (float)left : left != left ? NAN : 0.0f;
         mass = (float)sum;
     }

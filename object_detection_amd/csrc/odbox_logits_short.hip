@@ -261,9 +261,10 @@ __global__ __launch_bounds__(SHORT_THREADS) void score_grad_short_kernel(ScoreGr
 // Losses (out_rows), the gradient (GRAD) or both.  Each group has C words of LDS: -1 for a class off the list, for a listed class
 // first the number of its entry (a class listed twice shows by the entries that do not find theirs), then its q.
 // 392 832 x 80 float16, eight listed: losses 25 us, gradient 38 us (130 MB between them, 3.4 TB/s for the gradient): the chain list, logits there,
-// sums, LDS is waited for more than memory is.
+// sums, LDS is waited for more than memory is.  (The bound on registers: 16-bit bucket gradients of 24 values a lane took 110 without it, so
+// that four blocks a CU ran instead of five: 392 832 x 80 float16 62 -> 68 us.)
 template <class E, int L, int S, bool BUCKET, bool GRAD>
-__global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArgs a)
+__global__ __launch_bounds__(SHORT_THREADS, BUCKET && GRAD && E::VEC == 8 ? 8 - S : 1) void distill_short_kernel(DistillArgs a)
 {
     using Row = ShortRow<E, L, S>;
     constexpr uint32_t RB = SHORT_THREADS / L;
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(SHORT_THREADS) void distill_short_kernel(DistillArg
             }
         } else {
             double sum = 0.0;
-            for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), sum += (double)exp_split(t);
+            for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), sum += exp_wide(t);
 #pragma unroll
             for (int off = 1; off < L; off <<= 1) sum += __shfl_xor(sum, off);
             const double left = 1.0 - sum;
