@@ -935,16 +935,19 @@ __device__ __forceinline__ void load_and_prepare(const DistillArgs &a, size_t ro
 
 // What follows once the streamed classes' statistics are there; the same in every thread.
 struct ListTerms {
-    float m, l2;         // all classes; m = -inf: none has any probability
+    float m, l2;         // all classes; m = -inf: none has any probability; NaN: so is the row
     float mass;          // sum q (+ q0)
     float dense;         // the gradient off the list, over coefficient and softmax of the streamed classes
-    float rest;          // the bucket's part of the loss
+    float rest;          // the bucket's part of the loss; NaN for a row that is
 };
 __device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, const RowStats &st, const LogitsLds &sh)
 {
     const float mass = sh.sum[0], q0 = sh.sum[1], top = sh.sum[2], s_on = sh.sum[3];
     ListTerms r = {st.m, st.l2, mass, mass, 0.0f};
-    if (!a.bucket) return r;
+    if (!a.bucket) {
+        if (st.m != st.m) r.rest = NAN;          // also where nothing is listed
+        return r;
+    }
     const bool rest = st.m > -INFINITY;          // the bucket takes part
     if (rest) r.mass = mass + q0;
     r.m = vmax(st.m, top);
@@ -958,7 +961,7 @@ __device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, const RowS
         if (rest) r.rest = b.rest;
         if (q0 != q0) r.rest = q0;
     }
-    if (st.m != st.m || s_on != s_on) r.m = NAN;
+    if (st.m != st.m || s_on != s_on) r.m = r.rest = NAN;
     return r;
 }
 

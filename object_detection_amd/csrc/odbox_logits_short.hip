@@ -382,6 +382,7 @@ __global__ __launch_bounds__(SHORT_THREADS, BUCKET && GRAD && E::VEC == 8 ? 8 - 
                 list[id] = sum;
             }
         }
+        if (m != m) loss = m;                                // also where nothing is listed
         const bool dead = m == -INFINITY;
         if (a.out_rows) {
             loss += group_sum<L>(terms);
@@ -396,12 +397,13 @@ __global__ __launch_bounds__(SHORT_THREADS, BUCKET && GRAD && E::VEC == 8 ? 8 - 
                 r.zero(out);
             } else {
                 const float coef = w * a.t * a.scale * (a.up ? a.up[a.up_rows ? row : 0] : 1.0f);
+                const float none = m != m ? m : 0.0f;        // off the list where nothing there has a probability
                 r.store(out, [&](int k, int e, float v) {
                     const float b = list[r.base(k) + e];
                     if (!BUCKET) return coef * (exp2_hw((v - st.m) * a.c - st.l2) * mass - (b < 0.0f ? 0.0f : b));
                     const bool on = b >= 0.0f || b != b;
                     const float p = exp2_hw((v - (on ? m : st.m)) * a.c - (on ? l2 : st.l2));
-                    return on ? coef * (p * mass - b) : rest ? coef * dense * p : 0.0f;
+                    return on ? coef * (p * mass - b) : rest ? coef * dense * p : none;
                 });
             }
             fence();

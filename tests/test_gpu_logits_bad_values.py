@@ -1,0 +1,63 @@
+"""GPU tests of metric.distill_loss on rows that hold a NaN or an infinity: their loss and their whole gradient are NaN, the other rows' are not."""
+import pytest
+import torch
+
+from object_detection_amd import metric as M
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+INF, NAN = float('inf'), float('nan')
+# lanes, a wave, a block, segments of a row; whole rows with their gradient
+SHAPES = [(8, 7), (8, 80), (8, 700), (8, 2000), (8, 5000), (8, 70001), (520, 2500), (520, 9000)]
+
+
+def _inputs(rows, C, K, dtype):
+    gen = torch.Generator().manual_seed(C + K)
+    x = torch.randn(rows, C, generator=gen)
+    r = M.label_logprobs(x.cuda() + torch.randn(rows, C, generator=gen).cuda(), top_k=K)
+    return x.to(dtype).cuda(), r.top_logprobs, r.top_labels
+
+
+def _both_ways(x, tl, ids, rest):
+    """Losses and gradients of one call, and of a forward and a backward call."""
+    kw = dict(rest=rest, reduction=None)
+    yield M.distill_loss(x, tl, ids, return_grad=True, **kw)
+    leaf = x.clone().requires_grad_()
+    loss = M.distill_loss(leaf, tl, ids, **kw)
+    yield loss.detach(), torch.autograd.grad(loss.sum(), leaf)[0]
+    yield M.distill_loss(x, tl, ids, **kw), None
+
+
+def _check(x, tl, ids, rest, bad):
+    for loss, grad in _both_ways(x, tl, ids, rest):
+        want = torch.zeros(len(x), dtype=torch.bool)
+        want[bad] = True
+        assert torch.isnan(loss).tolist() == want.tolist(), (rest, loss[:8])
+        if grad is not None:
+            nan = torch.isnan(grad).cpu()
+            assert nan[want].all(), (rest, 'numbers in a bad row', nan[want].sum(1).tolist())
+            assert not nan[~want].any(), (rest, 'NaN in a good row')
+
+
+@pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,C', SHAPES)
+def test_bad_logits_where_nothing_is_listed(rows, C, dtype, rest):
+    x, tl, ids = _inputs(rows, C, 3, dtype)
+    ids[:2] = -1
+    tl[2:4] = -INF
+    ids[4] = -1                                                 # a good row without a list
+    tl[5] = -INF
+    off = [next(c for c in (0, 1, 2, 3) if c not in row) for row in ids[:4].tolist()]
+    for i, v in enumerate((NAN, INF, NAN, INF)):
+        x[i, off[i]] = v
+    _check(x, tl, ids, rest, [0, 1, 2, 3])
+
+
+@pytest.mark.parametrize('dtype', [F32, F16])
+@pytest.mark.parametrize('rows,C', SHAPES)
+def test_gradient_of_a_bucket_row_with_bad_logits_off_the_list(rows, C, dtype):
+    x, tl, ids = _inputs(rows, C, 3, dtype)
+    off = [next(c for c in (C - 1, C - 2, C - 3, C - 4) if c not in row) for row in ids[:2].tolist()]
+    x[0, off[0]], x[1, off[1]] = NAN, INF
+    _check(x, tl, ids, 'bucket', [0, 1])
