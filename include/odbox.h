@@ -340,6 +340,7 @@ int odbox_label_logprobs_backward(const void *logits, int dtype, size_t rows, in
  * ODBOX_REST_RENORMALISE: q is renormalised over the list (any common shift of the teacher's values cancels), rest = 0.
  * ODBOX_REST_BUCKET: q = exp(teacher_logprobs) and all classes off the list form one more class:
  *   rest = q0 (log q0 - log p0), q0 = max(0, 1 - sum q), p0 = the student's mass off the list; left out where the student has none.
+ * A listed teacher value that is NaN or +inf gives NaN like one of the logits; a list of nothing but -inf is as one without classes (q = 0).
  * row_weights w [rows] or NULL (all 1); a row of weight 0 is ignored: its logits are not read, its loss and gradient are 0.
  * out_rows [rows] or NULL: the row losses.  out_loss [1] or NULL: scale * their sum, summed in a fixed order (not both NULL).
  * grad [rows, C] or NULL: the gradient of scale * the sum, of the logits' dtype, contiguous; it may not overlap the logits.

@@ -858,15 +858,15 @@ __device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEnt
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (one wave's LDS accesses stay in order)
     float mass, q0 = 0.0f;
     if (!a.bucket) {
-        const float tm = wave_max(vmax(en.t[0], en.t[1]));
+        const float tm = wave_max(vmax(en.t[0], en.t[1])), about = tm > -INFINITY ? tm : 0.0f;
         float e[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) e[h] = on[h] && tm > -INFINITY ? exp2_hw((en.t[h] - tm) * LOG2E) : 0.0f;
+        for (int h = 0; h < 2; ++h) e[h] = on[h] ? exp2_hw((en.t[h] - about) * LOG2E) : 0.0f;
         const float tt = wave_sum(e[0] + e[1]), logt = LN2 * log2_hw(tt);
-        mass = tm > -INFINITY ? 1.0f : 0.0f;
+        mass = tt == 0.0f ? 0.0f : tt == tt ? 1.0f : NAN;    // the maximum does not see a NaN, the sum does
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            if (tm > -INFINITY) q[h] = e[h] / tt, logq[h] = (en.t[h] - tm) - logt;
+            if (tt != 0.0f) q[h] = e[h] / tt, logq[h] = (en.t[h] - about) - logt;
     } else {
         double sum = 0.0;
 #pragma unroll
@@ -944,24 +944,22 @@ __device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, const RowS
 {
     const float mass = sh.sum[0], q0 = sh.sum[1], top = sh.sum[2], s_on = sh.sum[3];
     ListTerms r = {st.m, st.l2, mass, mass, 0.0f};
-    if (!a.bucket) {
-        if (st.m != st.m) r.rest = NAN;          // also where nothing is listed
-        return r;
+    if (a.bucket) {
+        const bool rest = st.m > -INFINITY;      // the bucket takes part
+        if (rest) r.mass = mass + q0;
+        r.m = vmax(st.m, top);
+        r.l2 = -INFINITY;
+        if (r.m > -INFINITY) {
+            const float off = rest ? st.s * exp2_hw((st.m - r.m) * a.c) : 0.0f;
+            const float on = top > -INFINITY ? s_on * exp2_hw((top - r.m) * a.c) : 0.0f;
+            r.l2 = log2_hw(on + off);
+            const BucketTerms b = bucket_terms(on, off, mass, q0, (st.m - r.m) * a.inv_t + LN2 * (st.l2 - r.l2));
+            r.dense = b.dense;
+            if (rest) r.rest = b.rest;
+        }
     }
-    const bool rest = st.m > -INFINITY;          // the bucket takes part
-    if (rest) r.mass = mass + q0;
-    r.m = vmax(st.m, top);
-    r.l2 = -INFINITY;
-    if (r.m > -INFINITY) {
-        const float off = rest ? st.s * exp2_hw((st.m - r.m) * a.c) : 0.0f;
-        const float on = top > -INFINITY ? s_on * exp2_hw((top - r.m) * a.c) : 0.0f;
-        r.l2 = log2_hw(on + off);
-        const BucketTerms b = bucket_terms(on, off, mass, q0, (st.m - r.m) * a.inv_t + LN2 * (st.l2 - r.l2));
-        r.dense = b.dense;
-        if (rest) r.rest = b.rest;
-        if (q0 != q0) r.rest = q0;
-    }
-    if (st.m != st.m || s_on != s_on) r.m = r.rest = NAN;
+    // a NaN or +inf among the logits, also where nothing is listed, or among the teacher's values, except for an empty row
+    if (st.m != st.m || s_on != s_on || (mass != mass && r.m > -INFINITY)) r.m = r.rest = NAN;
     return r;
 }
 
@@ -1136,7 +1134,7 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
         const ListTerms t = list_terms(a, st, sh);
         if (threadIdx.x < WAVE) loss_out(a, row, weight, st, t, sh);
         const float coef = weight * a.t * a.scale, dense = coef * t.dense;
-        const bool none = t.m == -INFINITY || st.m == -INFINITY;     // nothing has a probability, or nothing off the list
+        const bool none = t.m == -INFINITY || (st.m == -INFINITY && t.m == t.m);     // nothing has a probability, or nothing off the list
         auto value = [&](float v) { return none ? 0.0f : exp2_hw((v - st.m) * a.c - st.l2) * dense; };
         typename E::raw *to = out + span.head;
 #pragma unroll
@@ -1174,8 +1172,9 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(DistillArgs a)
         if (threadIdx.x < WAVE) load_and_prepare<E>(a, p.row, x, sh);
         __syncthreads();
         const float4 f = a.stats[p.row];
-        const RowStats st = {f.x, f.y, 0.0f, f.z};
+        RowStats st = {f.x, f.y, 0.0f, f.z};
         const ListTerms t = list_terms(a, st, sh);
+        if (t.m != t.m) st.m = t.m;                          // NaN off the list too, where nothing there has a probability
         const float coef = weight * a.t * a.scale * (a.up ? a.up[a.up_rows ? p.row : 0] : 1.0f);
         if (t.m == -INFINITY) {
             zero_classes<E, NT>(out, p.n);

@@ -322,18 +322,17 @@ __global__ __launch_bounds__(SHORT_THREADS, BUCKET && GRAD && E::VEC == 8 ? 8 - 
             st = short_stats<L, false>(a.c, [&](auto f) { r.each(f); });
 
         // the list's terms, as in list_terms()
-        float tm = -INFINITY, tt = 1.0f, mass = 0.0f, q0 = 0.0f, loss = 0.0f;
+        float about = 0.0f, tt = 0.0f, mass = 0.0f, q0 = 0.0f, loss = 0.0f;
         float m = st.m, l2 = st.l2, dense = 0.0f, t;
         bool rest = false;
         if (!BUCKET) {
+            float tm = -INFINITY;
             for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), tm = vmax(tm, t);
             tm = group_max<L>(tm);
-            if (tm > -INFINITY) {
-                tt = 0.0f;
-                for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), tt += exp2_hw((t - tm) * LOG2E);
-                tt = group_sum<L>(tt);
-                mass = 1.0f;
-            }
+            if (tm > -INFINITY) about = tm;
+            for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), tt += exp2_hw((t - about) * LOG2E);
+            tt = group_sum<L>(tt);
+            mass = tt == 0.0f ? 0.0f : tt == tt ? 1.0f : NAN;    // the maximum does not see a NaN, the sum does
         } else {
             double sum = 0.0;
             for (uint32_t j = r.lane; j < a.K; j += L) entry(j, t), sum += exp_wide(t);
@@ -359,17 +358,16 @@ __global__ __launch_bounds__(SHORT_THREADS, BUCKET && GRAD && E::VEC == 8 ? 8 - 
                 dense = b.dense;
                 if (rest) loss = b.rest;
             }
-            if (q0 != q0) loss = q0;
             if (st.m != st.m) m = st.m;
         }
-        auto q_of = [&](float v) { return BUCKET ? exp_split(v) : tm > -INFINITY ? exp2_hw((v - tm) * LOG2E) / tt : 0.0f; };
+        auto q_of = [&](float v) { return BUCKET ? exp_split(v) : tt != 0.0f ? exp2_hw((v - about) * LOG2E) / tt : 0.0f; };
         float terms = 0.0f;
         for (uint32_t j = r.lane, i = 0; j < a.K; j += L, ++i) {
             const uint32_t id = entry(j, t);
             if (id >= a.C) continue;
             const float q = q_of(t);
             if (a.out_rows && (q > 0.0f || q != q)) {
-                const float logq = BUCKET ? t : (t - tm) - LN2 * log2_hw(tt);
+                const float logq = BUCKET ? t : (t - about) - LN2 * log2_hw(tt);
                 terms += q * (logq - ((E::get(x[id]) - m) * a.inv_t - LN2 * l2));
             }
             if (GRAD && (own >> i & 1u)) {
@@ -382,6 +380,7 @@ __global__ __launch_bounds__(SHORT_THREADS, BUCKET && GRAD && E::VEC == 8 ? 8 - 
                 list[id] = sum;
             }
         }
+        if (mass != mass && m > -INFINITY) m = mass;         // a NaN or +inf among the teacher's values, except for an empty row
         if (m != m) loss = m;                                // also where nothing is listed
         const bool dead = m == -INFINITY;
         if (a.out_rows) {

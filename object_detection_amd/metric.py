@@ -365,7 +365,8 @@ def distill_loss(logits, teacher_logprobs, teacher_labels, temperature: float = 
 
     rest='renormalise': q is renormalised over the list and rest is 0 (a common shift of the teacher's values cancels, so the
     teacher's logits / T will do).  rest='bucket': q is taken as it is and all classes off the list form one more class,
-    rest = q0 (log q0 - log p0).  A row of weight 0 is ignored whatever it holds.
+    rest = q0 (log q0 - log p0).  A row of weight 0 is ignored whatever it holds.  Otherwise a NaN or +inf among its logits or its
+    listed teacher values makes a row's loss and whole gradient NaN (a row of logits that are all -inf gives 0).
 
     reduction 'sum' (default), 'mean' (over the rows; 0 for none) or anything else (e.g. None): the losses [...] themselves,
     float32.  Differentiable w.r.t. the logits (captures: as label_logprobs); return_grad=True instead returns (loss, gradient), the gradient in the

@@ -61,3 +61,30 @@ def test_gradient_of_a_bucket_row_with_bad_logits_off_the_list(rows, C, dtype):
     off = [next(c for c in (C - 1, C - 2, C - 3, C - 4) if c not in row) for row in ids[:2].tolist()]
     x[0, off[0]], x[1, off[1]] = NAN, INF
     _check(x, tl, ids, 'bucket', [0, 1])
+
+
+@pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('rows,C', SHAPES)
+def test_bad_values_of_the_teacher(rows, C, dtype, rest):
+    x, tl, ids = _inputs(rows, C, 4, dtype)
+    tl[0] = NAN
+    tl[1, 2] = NAN
+    tl[2, 0] = INF
+    tl[3, 1:] = -INF
+    tl[3, 3] = NAN
+    ids[4, 2], tl[4, 2] = -1, NAN                               # an unused place may hold anything
+    ids[5], tl[5] = -1, NAN
+    tl[6] = -INF                                                # nothing is likely: a list without probability
+    x[7], tl[7] = -INF, NAN                                     # an empty row stays 0
+    _check(x, tl, ids, rest, [0, 1, 2, 3])
+
+
+@pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
+@pytest.mark.parametrize('C', [80, 30000])
+def test_scores_of_a_bad_teacher_row_reach_the_loss(C, rest):
+    teacher = torch.randn(8, C, generator=torch.Generator().manual_seed(C)).cuda()
+    teacher[1, 5], teacher[3, 7] = NAN, INF
+    r = M.label_logprobs(teacher, top_k=6)
+    x = torch.randn(8, C, generator=torch.Generator().manual_seed(1)).cuda()
+    _check(x, r.top_logprobs, r.top_labels, rest, [1, 3])
