@@ -919,8 +919,8 @@ __device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEnt
     float top = -INFINITY, s = 0.0f;
     if (a.bucket) {
         top = wave_max(vmax(first[0] ? en.x[0] : -INFINITY, first[1] ? en.x[1] : -INFINITY));
-        if (top > -INFINITY)
-            s = wave_sum((first[0] ? exp2_hw((en.x[0] - top) * a.c) : 0.0f) + (first[1] ? exp2_hw((en.x[1] - top) * a.c) : 0.0f));
+        const float about = top > -INFINITY ? top : 0.0f;    // (a maximum of NaNs alone is -inf as well, their sum is NaN)
+        s = wave_sum((first[0] ? exp2_hw((en.x[0] - about) * a.c) : 0.0f) + (first[1] ? exp2_hw((en.x[1] - about) * a.c) : 0.0f));
     }
     if (lane == 0) sh.sum[0] = mass, sh.sum[1] = q0, sh.sum[2] = top, sh.sum[3] = s;
 }
@@ -959,7 +959,7 @@ __device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, const RowS
         }
     }
     // a NaN or +inf among the logits, also where nothing is listed, or among the teacher's values, except for an empty row
-    if (st.m != st.m || s_on != s_on || (mass != mass && r.m > -INFINITY)) r.m = r.rest = NAN;
+    if (st.m != st.m || s_on != s_on || (mass != mass && r.m > -INFINITY)) r.m = r.dense = r.rest = NAN;
     return r;
 }
 

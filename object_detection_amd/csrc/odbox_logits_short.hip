@@ -347,18 +347,19 @@ __global__ __launch_bounds__(SHORT_THREADS, BUCKET && GRAD && E::VEC == 8 ? 8 - 
                 if (own >> i & 1u) top = vmax(top, E::get(x[ids[j]]));
             top = group_max<L>(top);
             m = vmax(st.m, top);
+            const float to = m > -INFINITY ? m : 0.0f;
+            float on = 0.0f;
+            for (uint32_t j = r.lane, i = 0; j < a.K; j += L, ++i)
+                if (own >> i & 1u) on += exp2_hw((E::get(x[ids[j]]) - to) * a.c);
+            on = group_sum<L>(on);
             if (m > -INFINITY) {
                 const float off = rest ? st.s * exp2_hw((st.m - m) * a.c) : 0.0f;
-                float on = 0.0f;
-                for (uint32_t j = r.lane, i = 0; j < a.K; j += L, ++i)
-                    if (own >> i & 1u) on += exp2_hw((E::get(x[ids[j]]) - m) * a.c);
-                on = group_sum<L>(on);
                 l2 = log2_hw(on + off);
                 const BucketTerms b = bucket_terms(on, off, (float)sum, q0, (st.m - m) * a.inv_t + LN2 * (st.l2 - l2));
                 dense = b.dense;
                 if (rest) loss = b.rest;
             }
-            if (st.m != st.m) m = st.m;
+            if (st.m != st.m || on != on) m = NAN;           // (the maxima do not see a NaN)
         }
         auto q_of = [&](float v) { return BUCKET ? exp_split(v) : tt != 0.0f ? exp2_hw((v - about) * LOG2E) / tt : 0.0f; };
         float terms = 0.0f;

@@ -88,3 +88,28 @@ def test_scores_of_a_bad_teacher_row_reach_the_loss(C, rest):
     r = M.label_logprobs(teacher, top_k=6)
     x = torch.randn(8, C, generator=torch.Generator().manual_seed(1)).cuda()
     _check(x, r.top_logprobs, r.top_labels, rest, [1, 3])
+
+
+@pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
+@pytest.mark.parametrize('dtype', [F32, F16])
+@pytest.mark.parametrize('K', [1, 3])
+@pytest.mark.parametrize('rows,C', SHAPES)
+def test_bad_logits_at_listed_classes(rows, C, K, dtype, rest):
+    x, tl, ids = _inputs(rows, C, K, dtype)
+    at = ids.long()
+    for i, v in enumerate((NAN, INF, NAN, INF, NAN)):
+        if i in (2, 3):
+            x[i] = -INF                                         # and nothing has a probability off the list
+        x[i, at[i]] = v                                         # every listed class
+    tl[4] = -INF                                                # of which the teacher needs none
+    x[5, at[5, 0]] = NAN                                        # one of them
+    _check(x, tl, ids, rest, [0, 1, 2, 3, 4, 5])
+
+
+@pytest.mark.parametrize('rest', ['renormalise', 'bucket'])
+@pytest.mark.parametrize('C', [1, 3, 100])
+def test_bad_logits_where_every_class_is_listed(C, rest):
+    x, tl, ids = _inputs(8, C, C, F32)
+    x[0], x[1], x[2, C - 1], x[3, 0] = NAN, INF, NAN, INF
+    x[4] = -INF
+    _check(x, tl, ids, rest, [0, 1, 2, 3])
