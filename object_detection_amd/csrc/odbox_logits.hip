@@ -847,7 +847,7 @@ struct ListEntries {
 
 // Fills sh.id (first entries of their classes; -1 otherwise), sh.val (a class's q, summed over its entries), sh.x (the student's
 // logits there), sh.q and sh.logq (by entry) and sh.sum: sum q, q0, and for the bucket the listed classes' maximum and sum about it.
-__device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEntries &en, LogitsLds &sh)
+__device__ __forceinline__ void prepare_list(const DistillArgs &a, bool bucket, const ListEntries &en, LogitsLds &sh)
 {
     const uint32_t lane = threadIdx.x;
     const bool on[2] = {en.id[0] >= 0, en.id[1] >= 0};
@@ -857,7 +857,7 @@ __device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEnt
     if (lane < 3) sh.id[128 + lane] = -1;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (one wave's LDS accesses stay in order)
     float mass, q0 = 0.0f;
-    if (!a.bucket) {
+    if (!bucket) {
         const float tm = wave_max(vmax(en.t[0], en.t[1])), about = tm > -INFINITY ? tm : 0.0f;
         float e[2];
 #pragma unroll
@@ -917,7 +917,7 @@ __device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEnt
             if (!first[h]) sh.id[lane + 64 * h] = -1;
     }
     float top = -INFINITY, s = 0.0f;
-    if (a.bucket) {
+    if (bucket) {
         top = wave_max(vmax(first[0] ? en.x[0] : -INFINITY, first[1] ? en.x[1] : -INFINITY));
         const float about = top > -INFINITY ? top : 0.0f;    // (a maximum of NaNs alone is -inf as well, their sum is NaN)
         s = wave_sum((first[0] ? exp2_hw((en.x[0] - about) * a.c) : 0.0f) + (first[1] ? exp2_hw((en.x[1] - about) * a.c) : 0.0f));
@@ -925,12 +925,12 @@ __device__ __forceinline__ void prepare_list(const DistillArgs &a, const ListEnt
     if (lane == 0) sh.sum[0] = mass, sh.sum[1] = q0, sh.sum[2] = top, sh.sum[3] = s;
 }
 template <class E>
-__device__ __forceinline__ void load_and_prepare(const DistillArgs &a, size_t row, const typename E::raw *x, LogitsLds &sh)
+__device__ __forceinline__ void load_and_prepare(const DistillArgs &a, bool bucket, size_t row, const typename E::raw *x, LogitsLds &sh)
 {
     ListEntries en;
     en.load_list(a, row);
     en.load_logits<E>(a, x);
-    prepare_list(a, en, sh);
+    prepare_list(a, bucket, en, sh);
 }
 
 // What follows once the streamed classes' statistics are there; the same in every thread.
@@ -940,11 +940,11 @@ struct ListTerms {
     float dense;         // the gradient off the list, over coefficient and softmax of the streamed classes
     float rest;          // the bucket's part of the loss; NaN for a row that is
 };
-__device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, const RowStats &st, const LogitsLds &sh)
+__device__ __forceinline__ ListTerms list_terms(const DistillArgs &a, bool bucket, const RowStats &st, const LogitsLds &sh)
 {
     const float mass = sh.sum[0], q0 = sh.sum[1], top = sh.sum[2], s_on = sh.sum[3];
     ListTerms r = {st.m, st.l2, mass, mass, 0.0f};
-    if (a.bucket) {
+    if (bucket) {
         const bool rest = st.m > -INFINITY;      // the bucket takes part
         if (rest) r.mass = mass + q0;
         r.m = vmax(st.m, top);
@@ -1038,15 +1038,15 @@ __global__ __launch_bounds__(NT, BUCKET ? 6 : 8) void distill_kernel(DistillArgs
         }
         const Span<E> span(x + p.first, p.n);
         if (BUCKET) mask_listed<E, NT>(a, p.row, p.first, span, mask);
-        if (a.segs == 1 && threadIdx.x < WAVE) load_and_prepare<E>(a, p.row, x, sh);
+        if (a.segs == 1 && threadIdx.x < WAVE) load_and_prepare<E>(a, BUCKET, p.row, x, sh);
         const Running r = scan_classes<E, NT, false, BUCKET, PASSING>(x + p.first, span, a.c, mask);
         const float3 j = block_join<NT>(r, a.c, sh);
         if (a.segs > 1) {
             if (threadIdx.x == 0) a.part[w] = make_float4(j.x, j.y, 0.0f, 0.0f);
             continue;
         }
-        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
-        const ListTerms t = list_terms(a, st, sh);
+        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, BUCKET ? a.K : 0, sh);
+        const ListTerms t = list_terms(a, BUCKET, st, sh);
         if (threadIdx.x < WAVE) loss_out(a, p.row, weight, st, t, sh);
         __syncthreads();
     }
@@ -1070,13 +1070,13 @@ __global__ __launch_bounds__(WAVE) void distill_join_kernel(DistillArgs a)
             const float3 two[2] = {share, make_float3(p.x, p.y, 0.0f)};
             share = join(two, 2, a.c);
         }
-        load_and_prepare<E>(a, row, x, sh);
+        load_and_prepare<E>(a, a.bucket, row, x, sh);
         const float M = wave_max(share.x);
         const float s = wave_sum(share.y != 0.0f ? share.y * exp2_hw((share.x - M) * a.c) : 0.0f);
         __syncthreads();
         const float3 j = make_float3(M, s, 0.0f);
         const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, WAVE>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
-        loss_out(a, row, weight, st, list_terms(a, st, sh), sh);
+        loss_out(a, row, weight, st, list_terms(a, a.bucket, st, sh), sh);
         __syncthreads();
     }
 }
@@ -1086,6 +1086,8 @@ __global__ __launch_bounds__(WAVE) void distill_join_kernel(DistillArgs a)
 // Reads go around the caches, and writes where rows are long: 444 -> 431 us, 1024 rows 142 -> 128, 4096 x 30000 120 -> 104.
 // 4096 x 131072 bfloat16: 423 us for 2.08 GB, 4.9 TB/s, what a copy of this size reaches.  One block of 1024 threads fills a CU's registers, so
 // rows go in rounds of 256: 777 x 50021 float32 take 86 us, four rounds for what would fit into 3.04.
+// The list's terms take the form from the arguments: with BUCKET in its place the registers come out worse (renormalised 50 000 x 4000 bfloat16
+// 187 -> 198 us, bucket 6000 x 30000 172 -> 178), where distill_kernel gains by it (2048 x 32768 float32 45.8 -> 41.4).
 template <class E, int NT, bool BUCKET>
 __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
 {
@@ -1128,10 +1130,10 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(DistillArgs a)
         if (BUCKET && reg.tid < span.edges && mask[M::words(span.nvec) - 1] >> reg.tid & 1u) edge = -INFINITY;
         absorb<1, false>(&edge, a.c, run);
         reg.forget();
-        if (threadIdx.x < WAVE) prepare_list(a, en, sh);
+        if (threadIdx.x < WAVE) prepare_list(a, a.bucket, en, sh);
         const float3 j = block_join<NT>(run, a.c, sh);
-        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, a.bucket ? a.K : 0, sh);
-        const ListTerms t = list_terms(a, st, sh);
+        const RowStats st = row_ok(j) ? stats_of(j) : careful_stats<E, NT>(x, a.C, a.c, BUCKET ? a.K : 0, sh);
+        const ListTerms t = list_terms(a, a.bucket, st, sh);
         if (threadIdx.x < WAVE) loss_out(a, row, weight, st, t, sh);
         const float coef = weight * a.t * a.scale, dense = coef * t.dense;
         const bool none = t.m == -INFINITY || (st.m == -INFINITY && t.m == t.m);     // nothing has a probability, or nothing off the list
@@ -1169,11 +1171,11 @@ __global__ __launch_bounds__(NT) void distill_grad_kernel(DistillArgs a)
             zero_classes<E, NT>(out, p.n);
             continue;
         }
-        if (threadIdx.x < WAVE) load_and_prepare<E>(a, p.row, x, sh);
+        if (threadIdx.x < WAVE) load_and_prepare<E>(a, a.bucket, p.row, x, sh);
         __syncthreads();
         const float4 f = a.stats[p.row];
         RowStats st = {f.x, f.y, 0.0f, f.z};
-        const ListTerms t = list_terms(a, st, sh);
+        const ListTerms t = list_terms(a, a.bucket, st, sh);
         if (t.m != t.m) st.m = t.m;                          // NaN off the list too, where nothing there has a probability
         const float coef = weight * a.t * a.scale * (a.up ? a.up[a.up_rows ? p.row : 0] : 1.0f);
         if (t.m == -INFINITY) {
