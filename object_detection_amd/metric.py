@@ -16,6 +16,7 @@ import contextlib
 import typing
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -134,6 +135,9 @@ def _logits(x):
     """Logits on their own GPU (host data: on the current one) in float32 / float16 / bfloat16; other types become float32."""
     if not isinstance(x, torch.Tensor):
         x = torch.as_tensor(x)
+    # the level first: unpack_dual alone costs 0.8 us
+    if getattr(forward_ad, '_current_level', 0) >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise NotImplementedError('class-logit operators have no forward-mode derivative')
     if not (x.is_cuda and x.dtype in _DTYPE_CODE):
         dev = x.device if x.is_cuda else _lib.require_gpu()
         x = x.to(device=dev, dtype=x.dtype if x.dtype in _DTYPE_CODE else torch.float32, non_blocking=True)
@@ -292,7 +296,7 @@ def label_logprobs(logits, labels=None, top_k: int = 0, temperature: float = 1.0
     w.r.t. the logits through logprobs, entropy and top_logprobs (odbox_label_logprobs_backward; the gradient has the logits'
     type; inside a graph capture, differentiate w.r.t. a leaf made there, logits.detach().requires_grad_(): a leaf of a live
     eager graph ties the capture to that graph's stream).  A logit of -inf is a forbidden class; a row of nothing else gives log-probabilities -inf, entropy 0 and no
-    gradient; a NaN or +inf makes its row NaN.  On a teacher, `top_logprobs` / `top_labels` are what `distill_loss` takes."""
+    gradient; a NaN or +inf makes its row NaN.  Logits with a forward-mode tangent are refused.  On a teacher, `top_logprobs` / `top_labels` are what `distill_loss` takes."""
     x = _logits(logits)
     temperature = _temperature(temperature)
     top_k = int(top_k)
@@ -369,7 +373,8 @@ def distill_loss(logits, teacher_logprobs, teacher_labels, temperature: float = 
     listed teacher values makes a row's loss and whole gradient NaN (a row of logits that are all -inf gives 0).
 
     reduction 'sum' (default), 'mean' (over the rows; 0 for none) or anything else (e.g. None): the losses [...] themselves,
-    float32.  Differentiable w.r.t. the logits (captures: as label_logprobs); return_grad=True instead returns (loss, gradient), the gradient in the
+    float32.  Differentiable w.r.t. the logits alone, the teacher's values and the weights being constants (captures and forward-mode
+    tangents: as label_logprobs); return_grad=True instead returns (loss, gradient), the gradient in the
     logits' type from the same call -- one pass over the logits where autograd takes two -- of the reduced loss, or for
     un-reduced losses of each row's loss w.r.t. that row."""
     x = _logits(logits)
