@@ -131,6 +131,13 @@ MAX_LOGITS = 1 << 24                                                        # OD
 _REST = {'renormalise': 0, 'bucket': 1}                                     # ODBOX_REST_*
 
 
+def _to(x, device, dtype):
+    """x on the device.  Copies of host data are waited for: one from pinned memory would still be under way when the call returns, and the
+    caller may write there.  A capture cannot wait; its replays read the host memory as it is then."""
+    at_once = x.is_cuda or (device.type == 'cuda' and torch.cuda.is_current_stream_capturing())
+    return x.to(device=device, dtype=dtype, non_blocking=at_once)
+
+
 def _logits(x):
     """Logits on their own GPU (host data: on the current one) in float32 / float16 / bfloat16; other types become float32."""
     if not isinstance(x, torch.Tensor):
@@ -140,7 +147,7 @@ def _logits(x):
         raise NotImplementedError('class-logit operators have no forward-mode derivative')
     if not (x.is_cuda and x.dtype in _DTYPE_CODE):
         dev = x.device if x.is_cuda else _lib.require_gpu()
-        x = x.to(device=dev, dtype=x.dtype if x.dtype in _DTYPE_CODE else torch.float32, non_blocking=True)
+        x = _to(x, dev, x.dtype if x.dtype in _DTYPE_CODE else torch.float32)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_LOGITS:
         raise ValueError('logits %r: the last axis holds 1..%d classes' % (tuple(x.shape), MAX_LOGITS))
     return x
@@ -172,7 +179,7 @@ def _side(x, dtype, device, shape, what):
         raise ValueError('%s %r does not fit the logits: expected %r' % (what, tuple(x.shape), tuple(shape)))
     if x.dtype == dtype and x.device == device and x.is_contiguous() and not x.requires_grad:
         return x
-    return x.detach().to(device=device, dtype=dtype, non_blocking=True).contiguous()
+    return _to(x.detach(), device, dtype).contiguous()
 
 
 def _class_ids(x, C, device, shape, what):
