@@ -54,3 +54,52 @@ def test_bucket_where_the_list_holds_nearly_everything(rows, C, K, T):
         R.within(float(loss[i]), want, le, 'loss of row %d' % i)
         for got in (grad, again):
             R.within(got[i].double().cpu().numpy(), wg, bound, 'gradient of row %d' % i)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('rows,C,K,pad', [(530, 2100, 128, 0), (600, 3001, 7, 5), (520, 9000, 33, 0), (530, 16001, 64, 2), (520, 33333, 5, 0),
+                                          (515, 65537, 20, 0), (515, 131073, 9, 0), (40, 80, 8, 0), (40, 1500, 30, 3)])
+def test_bucket_gradient_of_every_class_of_every_row(rows, C, K, pad, dtype):
+    """Against the formula in 64 bits on the device, with a bound that scales with each class's own gradient off the list.
+
+    Bound, with e, p0, q0 as above: p0 (sum q + q0) - q0 is off by p0 (2 e + 8 U) + q0 U, and where p0 > 1/2, as sum q less the
+    listed classes' mass, by that mass's (2 e + 4 U) and 2 U sum q; r_i and its products by (e + 8 U) relative; the result is rounded to its type.
+    At a listed class p and q are off by (2 e + 8 U) and (K + 8 + 4 |log q|) U relative."""
+    gen = torch.Generator().manual_seed(C)
+    x = torch.randn(rows, C + pad, generator=gen) * 2.0
+    x.scatter_add_(1, torch.randint(0, C, (rows, 6), generator=gen), torch.full((rows, 6), 6.0))
+    x = x.to(dtype).cuda()[:, :C]
+    teacher = x.float() + torch.randn(rows, C, generator=gen).cuda()
+    r = M.label_logprobs(teacher, top_k=K)
+    tl, ids = r.top_logprobs, r.top_labels
+    w = torch.rand(rows, generator=gen).cuda() + 0.5
+    if dtype == torch.float16:
+        w *= 2.0 ** 13                                          # as a step that scales its loss: keeps the gradients in float16's range
+    w[1::5] = 0.0
+    _, grad = M.distill_loss(x, tl, ids, rest='bucket', row_weights=w, reduction=None, return_grad=True)
+    leaf = x.detach().requires_grad_()
+    again, = torch.autograd.grad(M.distill_loss(leaf, tl, ids, rest='bucket', row_weights=w, reduction=None).sum(), leaf)
+
+    z = x.double()
+    z = z - z.amax(1, keepdim=True)
+    s = z.exp().sum(1, keepdim=True)
+    p = z.exp() / s
+    at = ids.long()
+    off = torch.ones_like(p, dtype=torch.bool).scatter_(1, at, False)
+    q = tl.double().exp()
+    q0, p0 = (1.0 - q.sum(1, keepdim=True)).clamp(min=0), torch.where(off, p, 0.0).sum(1, keepdim=True)
+    p_on = 1.0 - p0
+    weight = w.double()[:, None]
+    want = (p / p0 * (p0 - q0)).scatter(1, at, p.gather(1, at) - q) * weight
+    U = R.U
+    e = U * (4 * 1.4427 * -z.amin(1, keepdim=True) + 4 + R.adds(C) + 4 * s.log2())
+    dense = torch.where(p0 > 0.5, p_on * (2 * e + 4 * U) + 2 * U * q.sum(1, keepdim=True), p0 * (2 * e + 8 * U) + q0 * U) + (K + 4) * 2.0 ** -51
+    listed = p.gather(1, at) * (2 * e + 8 * U) + q * U * (K + 8 + 4 * tl.double().abs())
+    bound = (p / p0 * dense).scatter(1, at, listed) * weight + (e + 8 * U + R.EPS[dtype]) * want.abs() + R.TINY[dtype]
+    # the bound tells a class's gradient from 0 (which a vector left out would hold) nearly everywhere
+    seen = off & (weight > 0)
+    assert (bound[seen] < 0.5 * want[seen].abs()).double().mean() > 0.9
+    for g in (grad, again):
+        wrong = (g.double() - want).abs() > bound
+        assert not wrong.any(), (int(wrong.sum()), wrong.nonzero()[:4].tolist())
+        assert (g[1::5] == 0).all()
