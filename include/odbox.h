@@ -356,7 +356,7 @@ int odbox_distill_loss(const void *logits, int dtype, size_t rows, int C, size_t
                        float *out_stats /*[rows,4] or NULL*/, void *grad /*[rows,C] or NULL*/,
                        void *workspace, size_t workspace_bytes, void *stream);
 
-/* The gradient alone, from the forward call's statistics: scale * upstream * d loss[row] / d logits, upstream one device scalar
+/* The gradient alone, from the forward call's statistics (rows of up to 1536 float32 or 2048 16-bit classes compute them again): scale * upstream * d loss[row] / d logits, upstream one device scalar
  * (upstream_rows = 0) or one value a row (upstream_rows != 0). */
 int odbox_distill_loss_backward(const void *logits, int dtype, size_t rows, int C, size_t row_stride,
                                 const float *teacher_logprobs /*[rows,K]*/, const int32_t *teacher_labels /*[rows,K]*/, int K,

@@ -267,7 +267,9 @@ __device__ __forceinline__ void rank_candidates(uint32_t n, uint32_t k, const To
 }
 
 // The k (<= ODBOX_MAX_TOP, <= n) largest of n unique keys: the k-th key by a radix selection of eight bits a pass, then exactly k
-// keys are collected.  Right for every input, eight passes: where the threshold below keeps too few or too many candidates.
+// keys are collected.  Right for every input, eight passes: where the threshold below keeps too few or too many candidates.  That is also where a mask
+// leaves fewer than k classes of a row or segment, and it is slow: 4096 x 32768 bfloat16, 64 classes, 78 us with 99 % forbidden, 3 ms with
+// 99.9 %; 48 x 65537 float32, 20 classes, 20 and 139 us.
 // They end up in top.key in order.  (A call: key is a plain object.)
 template <int NT, class Key>
 __device__ __attribute__((noinline)) void top_radix(uint32_t n, uint32_t k, LogitsLds &sh, TopLds &top, Key key)
@@ -553,8 +555,8 @@ __device__ __forceinline__ Piece piece_of(size_t w, uint32_t segs, uint32_t seg,
 }
 
 // Without top classes: the row streams by, 64 or 128 bytes a thread in flight and 64 registers, so that eight blocks of 256 share a CU and
-// every row of a 2048-row call is under way at once.  2048 x 131072 bfloat16: 83 us, 6.5 TB/s; 7.4 vector instructions a value (widen,
-// maximum, multiply-add, exponential, two sums) keep the SIMDs 85 % busy, so it is bound by both.
+// every row of a 2048-row call is under way at once.  2048 x 131072 bfloat16: 83 us, 6.5 TB/s, where a kernel that only reads reaches 7.0; 7.4
+// vector instructions a value (widen, maximum, multiply-add, exponential, two sums), at four cycles each 50 us, more for the exponential.
 template <class E, int NT, bool PASSING>
 __global__ __launch_bounds__(NT, 8) void score_kernel(ScoreArgs a)
 {
@@ -577,8 +579,9 @@ __global__ __launch_bounds__(NT, 8) void score_kernel(ScoreArgs a)
 }
 
 // With top classes: the row stays in registers, and blocks stay for many rows: once a row's candidates are found, the next row
-// comes into the registers while they are ranked.  4096 x 32768 bfloat16, 64 classes: 78 us, 3.4 TB/s, bound by the vector unit (the scores'
-// 7.4 instructions a value, two more to look for candidates, about 150 a row and thread for threshold and ranking).
+// comes into the registers while they are ranked.  4096 x 32768 bfloat16, 64 classes: 78 us a pass, 3.4 TB/s, bound by the vector unit: 15.6
+// instructions a value by the counters, 53 us at four cycles.  The scores' 7.4, two to look for candidates and about 150 a row and thread for
+// threshold and ranking are 10.6 of them; where the others go is not known.
 template <class E, int NT>
 __global__ __launch_bounds__(NT, 4) void score_top_kernel(ScoreArgs a)
 {
@@ -724,7 +727,7 @@ __device__ void zero_classes(typename E::raw *out, uint32_t n)
 }
 
 // out = p (ga + gb log2 p) at n classes of a row, p by the row's statistics.  Reads and writes go around the caches (nobody asks for either
-// soon): 2048 x 131072 bfloat16 345 -> 312 us for the step.  Bound by memory: 186 us for 1 GB, 5.5 TB/s.
+// soon): 2048 x 131072 bfloat16 345 -> 312 us for the step.  Bound by memory: 186 us for 1.04 GB, 5.6 TB/s.
 template <class E, int NT, int U, bool ENT>
 __device__ __forceinline__ void write_grad(const RowStats &st, float ga, float gb, const typename E::raw *x, typename E::raw *out, uint32_t n, float c)
 {
@@ -1019,9 +1022,10 @@ __device__ __forceinline__ void listed_grad(const DistillArgs &a, float coef, co
 
 constexpr uint32_t MASK_CLASSES = 262144;        // of a bucket segment: 32 KB of mask
 
-// Losses, one block per row or per segment of a row: the row streams by.  2048 x 32768 float32: 46 us, 5.5 TB/s.  The bucket's mask costs a
-// word of LDS for every 32 values of a thread and, where a wave has a listed class in them, three more instructions a value, which hide
-// behind the reads: 2048 x 131072 bfloat16, 64 listed 117 us.  (Eight blocks a CU for it: 312 -> 326 us with the gradient.)
+// Losses, one block per row or per segment of a row: the row streams by.  2048 x 32768 float32: 41.5 us, 6.1 TB/s.  The bucket's mask costs a
+// word of LDS for every 32 values of a thread and, where a wave has a listed class in them, three more instructions a value: 2048 x
+// 131072 bfloat16 ahead of a gradient, 64 listed 115 us, 4.4 TB/s, the same without the mask; why it stays below the scores' rate is not
+// known.  (Eight blocks a CU for it: 312 -> 326 us with the gradient.)
 template <class E, int NT, bool BUCKET, bool PASSING>
 __global__ __launch_bounds__(NT, BUCKET ? 6 : 8) void distill_kernel(DistillArgs a)
 {
@@ -1084,8 +1088,8 @@ __global__ __launch_bounds__(WAVE) void distill_join_kernel(DistillArgs a)
 // Losses and gradient of whole rows that fit into a block's registers: one read, one write.  (Fetching the next row's vectors as this
 // row's gradients leave them was measured too: 4096 x 131072 bfloat16 433 -> 476 us.  Memory moves reads and writes faster apart.)
 // Reads go around the caches, and writes where rows are long: 444 -> 431 us, 1024 rows 142 -> 128, 4096 x 30000 120 -> 104.
-// 4096 x 131072 bfloat16: 423 us for 2.08 GB, 4.9 TB/s, what a copy of this size reaches.  One block of 1024 threads fills a CU's registers, so
-// rows go in rounds of 256: 777 x 50021 float32 take 86 us, four rounds for what would fit into 3.04.
+// 4096 x 131072 bfloat16: 427 us for 2.08 GB, 4.9 TB/s, what a copy of this size reaches.  One block of 1024 threads fills a CU's registers, so
+// rows go in rounds of 256: a pass over 768 x 50021 float32 takes 80 us, 769 rows 88, 777 rows 90 to 92, 1024 rows 103.
 // The list's terms take the form from the arguments: with BUCKET in its place the registers come out worse (renormalised 50 000 x 4000 bfloat16
 // 187 -> 198 us, bucket 6000 x 30000 172 -> 178), where distill_kernel gains by it (2048 x 32768 float32 45.8 -> 41.4).
 template <class E, int NT, bool BUCKET>
@@ -1241,8 +1245,9 @@ static Split split_rows(size_t rows, uint32_t C, uint32_t blocks, uint32_t most)
     return {(C + seg - 1) / seg, seg};
 }
 constexpr uint32_t FILL_BLOCKS = 1024;
-// Loss and gradient by whole rows from this many on: below, segments fill the chip better (rows of 50021 float32, both ways:
-// 300 rows 48 / 46 us, 520 rows 75 / 73, 777 rows 99 / 115; 520 rows of 9000 classes 30 / 33).
+// Loss and gradient by whole rows from this many on; few rows fill the chip better in segments.  Whole rows / segments, us a pass: bucket, 50021
+// float32 classes, 300 rows 45.4 / 45.2, 520 rows 69.1 / 67.2, 768 rows 80.3 / 89.3, 777 rows 92.5 / 91.4; renormalised 520 rows 60.1 / 66.0, 777 rows
+// 82.7 / 90.6; 520 rows of 9000 classes 17.0 / 24.5.  (Renormalised 200 rows take 23.0 / 32.8: the limit could be lower.)
 constexpr size_t FUSE_ROWS = 512;
 // What a block of NT threads holds in registers.
 static uint32_t resident(int dtype, int nt) { return 16u * nt * (dtype == ODBOX_DTYPE_F32 ? 4 : 8); }
@@ -1253,8 +1258,11 @@ static Split distill_split(size_t rows, uint32_t C)
 {
     return split_rows(rows, C, FILL_BLOCKS, MASK_CLASSES);
 }
-// Logits that the 256 MB Infinity Cache could not hold are read around the caches when nobody reads them again (no statistics are kept for
-// a gradient): 2048 x 131072 bfloat16 scores 99 -> 92 us, 2048 x 32768 float32 losses (256 MB) 51 -> 48 us.  Ahead of a gradient the same
+// Logits that pass by once (no statistics are kept for a gradient) are read around the caches from the Infinity Cache's own size on, 256 MB.
+// Below, it is a loss where they are still in the cache and a gain where they are not.  Cached / around, us, the same logits each time, and two sets of
+// them in turn: scores of 50021 bfloat16 classes, 96 MB 24.5 / 23.4 and 23.4 / 24.0; 192 MB 33.3 / 34.4 and 39.3 / 35.7; 240 MB 42.2 / 43.9 and 49.1 / 44.4;
+// 256 MB 44.7 / 46.0 and 51.4 / 46.6; 288 MB 50.0 / 50.0 and 56.2 / 51.2; 512 MB 94.8 / 85.7 and 94.0 / 86.2.  Losses of 32768 float32 classes, 192 MB 33.2 / 33.4
+// and 38.6 / 34.1; 256 MB 42.0 / 42.8 and 49.2 / 43.4; 512 MB 93.7 / 82.4 and 93.6 / 82.9.  Ahead of a gradient the same
 // loads cost what its second read then misses (1021 x 100003 float16 scores both ways 126 -> 146 us, 4600 rows still 590 -> 618); losses
 // gain where the cache holds little of them: both ways 300 x 1000003 bfloat16 (600 MB) 376 -> 384 us, 3600 x 100003 (720 MB) 455 ->
 // 442, 4000 x 131072 605 -> 554.
