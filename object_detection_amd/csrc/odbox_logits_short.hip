@@ -261,8 +261,8 @@ __global__ __launch_bounds__(SHORT_THREADS) void score_grad_short_kernel(ScoreGr
 // Losses (out_rows), the gradient (GRAD) or both.  Each group has C words of LDS: -1 for a class off the list, for a listed class
 // first the number of its entry (a class listed twice shows by the entries that do not find theirs), then its q.
 // 392 832 x 80 float16, eight listed, by autograd: losses 25 us, gradient 38 us (130 MB, 3.4 TB/s).  24 and 43 vector instructions a value, at four
-// cycles 15 and 27 us: the gradient launch computes maximum, sums and the teacher's softmax again.  (The bound on registers: 16-bit bucket gradients of 24 values a lane took 110 without it, so
-// that four blocks a CU ran instead of five: 392 832 x 80 float16 62 -> 68 us.)
+// cycles 15 and 27 us: the gradient launch computes maximum, sums and the teacher's softmax again.  (The bound on registers: 16-bit bucket
+// gradients of 24 values a lane took 110 without it, so that four blocks a CU ran instead of five: 392 832 x 80 float16 64 -> 68 us.)
 template <class E, int L, int S, bool BUCKET, bool GRAD>
 __global__ __launch_bounds__(SHORT_THREADS, BUCKET && GRAD && E::VEC == 8 ? 8 - S : 1) void distill_short_kernel(DistillArgs a)
 {
